@@ -214,7 +214,8 @@ def _quantised(x):
     """(codes, scale) of the rows of x: the largest finite magnitude of a row becomes 448."""
     x = x.float()
     top = x.abs().nan_to_num(0.0, 0.0, 0.0).amax(-1).clamp(min=FP8_FLOOR)
-    return (x * (FP8_MAX / top).unsqueeze(-1)).to(FP8), top / FP8_MAX
+    most = torch.full_like(top, FP8_MAX)           # number / tensor would be the number times a rounded reciprocal
+    return (x * (most / top).unsqueeze(-1)).to(FP8), top / most
 
 
 def _places(cu, n):
