@@ -1,0 +1,128 @@
+// Paged key/value cache, the attention over it and the verification of drafted tokens: C entry points, argument checks and launches
+// (kernels in paged_cache.h, paged_attn.h, draft_kernels.h).
+#include <string.h>
+
+#include "host_common.h"
+#include "draft_kernels.h"
+#include "paged_attn.h"
+
+using namespace fgrpo;
+
+namespace {
+
+int check_cache(const char* who, const fgrpo_paged_cache* c, const int32_t* table, long long table_st, int width, const int32_t* lens,
+                const int32_t* cu, int B, int T) {
+  if (!c || !c->k || !c->v || !lens || !cu) return fail(FGRPO_ERR_BAD_ARG, "%s: null argument", who);
+  if (B <= 0 || T <= 0 || width < 0 || (width > 0 && !table)) return fail(FGRPO_ERR_BAD_ARG, "%s: B=%d T=%d width=%d", who, B, T, width);
+  if (table_st < 0 || (table_st < width && B > 1)) return fail(FGRPO_ERR_BAD_ARG, "%s: rows of the block table %lld apart, %d wide", who, table_st, width);
+  if (c->num_blocks <= 0 || c->heads <= 0) return fail(FGRPO_ERR_BAD_ARG, "%s: num_blocks=%d heads=%d", who, c->num_blocks, c->heads);
+  if (c->block_size < 16 || c->block_size > 65536 || (c->block_size & (c->block_size - 1)))
+    return fail(FGRPO_ERR_UNSUPPORTED, "%s: block size %d (a power of two from 16 to 65536)", who, c->block_size);
+  if ((long long)width * c->block_size >= (1LL << 31)) return fail(FGRPO_ERR_UNSUPPORTED, "%s: a block table of %d blocks of %d reaches 2^31 tokens", who, width, c->block_size);
+  if (c->head_dim != 128 && c->head_dim != 64) return fail(FGRPO_ERR_UNSUPPORTED, "%s: head dimension %d not supported (128 or 64)", who, c->head_dim);
+  if (c->dtype != FGRPO_BF16 && c->dtype != FGRPO_F8E4M3) return fail(FGRPO_ERR_BAD_ARG, "%s: cache dtype=%d", who, c->dtype);
+  const bool fp8 = c->dtype == FGRPO_F8E4M3;
+  if (fp8 && (!c->k_scale || !c->v_scale)) return fail(FGRPO_ERR_BAD_ARG, "%s: an e4m3 cache has scales", who);
+  if (!aligned16(c->k) || !aligned16(c->v)) return fail(FGRPO_ERR_ALIGN, "%s: the cache must be 16-byte aligned", who);
+  for (int i = 0; i < 3; ++i) {
+    if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_stride[i] % 16 || c->v_stride[i] % 16)
+      return fail(FGRPO_ERR_ALIGN, "%s: strides of the cache must be multiples of 16 elements", who);
+    if (fp8 && (c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0)) return fail(FGRPO_ERR_BAD_ARG, "%s: negative stride", who);
+  }
+  return 0;
+}
+
+PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long table_st, int width, const int32_t* lens, const int32_t* cu, int B, int T) {
+  PagedView v;
+  memset(&v, 0, sizeof(v));
+  v.k = (char*)c->k, v.v = (char*)c->v, v.k_scale = c->k_scale, v.v_scale = c->v_scale;
+  for (int i = 0; i < 3; ++i)
+    v.k_st[i] = c->k_stride[i], v.v_st[i] = c->v_stride[i], v.ks_st[i] = c->k_scale_stride[i], v.vs_st[i] = c->v_scale_stride[i];
+  v.table = table, v.lens = lens, v.cu = cu, v.table_st = table_st;
+  v.B = B, v.T = T, v.width = width, v.page_log2 = __builtin_ctz(c->block_size), v.num_pages = c->num_blocks, v.Hkv = c->heads;
+  return v;
+}
+
+#define PAGED_DISPATCH(kernel, c, grid, threads, st, ...)                                                              \
+  do {                                                                                                                 \
+    const bool fp8_ = (c)->dtype == FGRPO_F8E4M3;                                                                      \
+    if ((c)->head_dim == 128 && fp8_) hipLaunchKernelGGL((kernel<128, true>), grid, dim3(threads), 0, st, __VA_ARGS__);  \
+    else if ((c)->head_dim == 128) hipLaunchKernelGGL((kernel<128, false>), grid, dim3(threads), 0, st, __VA_ARGS__);    \
+    else if (fp8_) hipLaunchKernelGGL((kernel<64, true>), grid, dim3(threads), 0, st, __VA_ARGS__);                      \
+    else hipLaunchKernelGGL((kernel<64, false>), grid, dim3(threads), 0, st, __VA_ARGS__);                               \
+    HIP_TRY(hipGetLastError());                                                                                        \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int fgrpo_paged_cache_write(const fgrpo_paged_cache* cache, const void* k, const void* v, long long k_stride_t, long long k_stride_h,
+                            long long v_stride_t, long long v_stride_h, const int32_t* block_table, long long table_stride, int width,
+                            const int32_t* seqused_k, const int32_t* cu_seqlens, int n_seq, int T, void* stream) {
+  const int rc = check_cache("paged_cache_write", cache, block_table, table_stride, width, seqused_k, cu_seqlens, n_seq, T);
+  if (rc) return rc;
+  if (!k || !v) return fail(FGRPO_ERR_BAD_ARG, "paged_cache_write: null argument");
+  if (!aligned16(k) || !aligned16(v)) return fail(FGRPO_ERR_ALIGN, "paged_cache_write: k/v must be 16-byte aligned");
+  const long long st[4] = {k_stride_t, k_stride_h, v_stride_t, v_stride_h};
+  for (int i = 0; i < 4; ++i)
+    if (st[i] < 0 || st[i] % 8) return fail(FGRPO_ERR_ALIGN, "paged_cache_write: strides must be multiples of 8 elements");
+  if (width == 0) return 0;      // no sequence has a place
+  PagedWrite p;
+  p.c = view_of(cache, block_table, table_stride, width, seqused_k, cu_seqlens, n_seq, T);
+  p.k = (const bf16_t*)k, p.v = (const bf16_t*)v, p.k_t = k_stride_t, p.k_h = k_stride_h, p.v_t = v_stride_t, p.v_h = v_stride_h;
+  PAGED_DISPATCH(paged_write_kernel, cache, dim3((T + 3) / 4), 256, (hipStream_t)stream, p);
+  return 0;
+}
+
+int fgrpo_paged_cache_read(const fgrpo_paged_cache* cache, const int32_t* block_table, long long table_stride, int width,
+                           const int32_t* seqused_k, const int32_t* cu_seqlens_k, int n_seq, int total, void* k_out, void* v_out, void* stream) {
+  const int rc = check_cache("paged_cache_read", cache, block_table, table_stride, width, seqused_k, cu_seqlens_k, n_seq, total);
+  if (rc) return rc;
+  if (!k_out || !v_out) return fail(FGRPO_ERR_BAD_ARG, "paged_cache_read: null argument");
+  if (!aligned16(k_out) || !aligned16(v_out)) return fail(FGRPO_ERR_ALIGN, "paged_cache_read: outputs must be 16-byte aligned");
+  if (width == 0) return 0;
+  PagedRead p;
+  p.c = view_of(cache, block_table, table_stride, width, seqused_k, cu_seqlens_k, n_seq, total);
+  p.k = (bf16_t*)k_out, p.v = (bf16_t*)v_out;
+  PAGED_DISPATCH(paged_read_kernel, cache, dim3((total + 3) / 4), 256, (hipStream_t)stream, p);
+  return 0;
+}
+
+int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride_h, const fgrpo_paged_cache* cache, const int32_t* block_table,
+                         long long table_stride, int width, const int32_t* seqused_k, const int32_t* cu_seqlens_q, int n_seq, int T, int Hq,
+                         float softmax_scale, int causal, void* out, float* lse, void* stream) {
+  const int rc = check_cache("paged_attn_fwd", cache, block_table, table_stride, width, seqused_k, cu_seqlens_q, n_seq, T);
+  if (rc) return rc;
+  if (!q || !out) return fail(FGRPO_ERR_BAD_ARG, "paged_attn_fwd: null argument");
+  if (Hq <= 0 || Hq % cache->heads) return fail(FGRPO_ERR_BAD_ARG, "paged_attn_fwd: Hq=%d Hkv=%d", Hq, cache->heads);
+  if (!(softmax_scale > 0.f)) return fail(FGRPO_ERR_BAD_ARG, "paged_attn_fwd: softmax scale must be positive");
+  if (!aligned16(q) || !aligned16(out)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: q/out must be 16-byte aligned");
+  if (q_stride_t < 0 || q_stride_h < 0 || q_stride_t % 8 || q_stride_h % 8)
+    return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: strides must be multiples of 8 elements");
+  const int G = Hq / cache->heads;
+  if ((long long)T * G >= (1LL << 31) - 256) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: T=%d rows of %d heads", T, G);
+  PagedAttn p;
+  p.c = view_of(cache, block_table, table_stride, width, seqused_k, cu_seqlens_q, n_seq, T);
+  p.q = (const bf16_t*)q, p.q_t = q_stride_t, p.q_h = q_stride_h, p.out = (bf16_t*)out, p.lse = lse;
+  p.scale = softmax_scale, p.Hq = Hq, p.G = G, p.causal = causal != 0;
+  const long long tiles = ((long long)T * G) / kPagedRows + n_seq;
+  if (cache->heads > 65535 || tiles >= (1LL << 31)) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: %lld tiles of %d heads", tiles, cache->heads);
+  PAGED_DISPATCH(paged_attn_kernel, cache, dim3((unsigned)tiles, cache->heads), 256, (hipStream_t)stream, p);
+  return 0;
+}
+
+int fgrpo_verify_drafts(const void* target, long long target_stride, const void* draft, long long draft_stride, int draft_rows, int dtype,
+                        const int64_t* ids, const float* u, const int32_t* cu_seqlens, int n_seq, int T, int V, int32_t* accepted, int64_t* tokens,
+                        void* stream) {
+  if (!target || !ids || !u || !cu_seqlens || !accepted || !tokens) return fail(FGRPO_ERR_BAD_ARG, "verify_drafts: null argument");
+  if (n_seq <= 0 || T <= 0 || V <= 0 || target_stride < V || draft_rows < 0 || (draft && draft_stride < V))
+    return fail(FGRPO_ERR_BAD_ARG, "verify_drafts: n_seq=%d T=%d V=%d, rows %lld and %lld apart", n_seq, T, V, target_stride, draft_stride);
+  if (dtype != FGRPO_BF16 && dtype != FGRPO_F32) return fail(FGRPO_ERR_BAD_ARG, "verify_drafts: dtype=%d", dtype);
+  VerifyParams p{target, draft, (const long long*)ids, u, cu_seqlens, target_stride, draft_stride, n_seq, T, V, dtype == FGRPO_F32, draft_rows, accepted, (long long*)tokens};
+  hipLaunchKernelGGL(verify_drafts_kernel, dim3(n_seq), dim3(1024), 0, (hipStream_t)stream, p);
+  HIP_TRY(hipGetLastError());
+  return 0;
+}
+
+}  // extern "C"

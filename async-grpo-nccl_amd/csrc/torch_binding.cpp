@@ -46,6 +46,10 @@ struct Api {
   FGRPO_ENTRY(fgrpo_varlen_attn_workspace_len);
   FGRPO_ENTRY(fgrpo_varlen_attn_fwd_len);
   FGRPO_ENTRY(fgrpo_varlen_attn_bwd_len);
+  FGRPO_ENTRY(fgrpo_paged_cache_write);
+  FGRPO_ENTRY(fgrpo_paged_cache_read);
+  FGRPO_ENTRY(fgrpo_paged_attn_fwd);
+  FGRPO_ENTRY(fgrpo_verify_drafts);
 } api;
 
 void init(const std::unordered_map<std::string, uint64_t>& at) {
@@ -76,6 +80,10 @@ void init(const std::unordered_map<std::string, uint64_t>& at) {
   FGRPO_SET(fgrpo_varlen_attn_workspace_len);
   FGRPO_SET(fgrpo_varlen_attn_fwd_len);
   FGRPO_SET(fgrpo_varlen_attn_bwd_len);
+  FGRPO_SET(fgrpo_paged_cache_write);
+  FGRPO_SET(fgrpo_paged_cache_read);
+  FGRPO_SET(fgrpo_paged_attn_fwd);
+  FGRPO_SET(fgrpo_verify_drafts);
 }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "fgrpo ", what, " failed (", rc, "): ", api.fgrpo_last_error()); }
@@ -459,6 +467,144 @@ Tensor varlen_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   return wanted ? VarlenAttention::apply(q, k, v, a) : VarlenAttention::forward(nullptr, q, k, v, a);
 }
 
+// ---- paged cache, the attention over it, verification of drafts: no gradients, so no nodes ------------------------------------
+void no_gradient(const Tensor& t, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined(), "fgrpo: ", what, " has no gradient: call it under torch.no_grad()");
+}
+// int32, contiguous, on the device of `like`; [n] or any length
+Tensor index_vector(const Tensor& t, const Tensor& like, const char* name, int64_t n = -1) {
+  TORCH_CHECK(t.dim() == 1 && (n < 0 || t.numel() == n), "fgrpo: ", name, " must have ", n < 0 ? std::string("one dimension") : std::to_string(n) + " entries", ", got ", t.sizes());
+  TORCH_CHECK(!t.is_floating_point() && t.scalar_type() != at::kBool, "fgrpo: ", name, " must hold whole numbers, got ", t.scalar_type());
+  require_one_gpu(like, t);
+  return t.to(at::kInt).contiguous();
+}
+
+struct PagedBatch {
+  fgrpo_paged_cache c;
+  Tensor table, lens, cu;
+  int B, width;
+  const int32_t* table_ptr() const { return width > 0 ? table.data_ptr<int32_t>() : nullptr; }
+};
+PagedBatch paged_batch(const Tensor& k, const Tensor& v, const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
+                       const Tensor& table, const Tensor& lens, const Tensor& cu) {
+  PagedBatch b;
+  TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "fgrpo: the cache is [num_blocks, block_size, heads, head_dim], got k ", k.sizes(), ", v ", v.sizes());
+  TORCH_CHECK(k.scalar_type() == v.scalar_type() && (k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat8_e4m3fn),
+              "fgrpo: a cache is bf16 or float8_e4m3fn, got k ", k.scalar_type(), ", v ", v.scalar_type());
+  TORCH_CHECK(k.size(0) > 0 && k.size(0) < (1LL << 31) && k.size(1) < (1LL << 31) && k.size(2) < (1LL << 31) && k.size(3) < (1LL << 31), "fgrpo: cache ", k.sizes());
+  TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "fgrpo: the cache's innermost dimension must be contiguous");
+  require_one_gpu(k, v);
+  memset(&b.c, 0, sizeof(b.c));
+  const bool fp8 = k.scalar_type() == at::kFloat8_e4m3fn;
+  const Tensor ks = opt(k_scale), vs = opt(v_scale);
+  TORCH_CHECK(fp8 == ks.defined() && fp8 == vs.defined(), "fgrpo: ", fp8 ? "an e4m3 cache needs k_scale and v_scale" : "a bf16 cache has no scales");
+  b.c.k = k.data_ptr(), b.c.v = v.data_ptr();
+  for (int i = 0; i < 3; ++i) b.c.k_stride[i] = k.stride(i), b.c.v_stride[i] = v.stride(i);
+  if (fp8) {
+    require_one_gpu(k, ks, vs);
+    for (const Tensor& s : {ks, vs})
+      TORCH_CHECK(s.scalar_type() == at::kFloat && s.sizes() == k.sizes().slice(0, 3), "fgrpo: scales are fp32 ", k.sizes().slice(0, 3), ", got ", s.scalar_type(), " ", s.sizes());
+    b.c.k_scale = ks.data_ptr<float>(), b.c.v_scale = vs.data_ptr<float>();
+    for (int i = 0; i < 3; ++i) b.c.k_scale_stride[i] = ks.stride(i), b.c.v_scale_stride[i] = vs.stride(i);
+  }
+  b.c.num_blocks = (int)k.size(0), b.c.block_size = (int)k.size(1), b.c.heads = (int)k.size(2), b.c.head_dim = (int)k.size(3);
+  b.c.dtype = fp8 ? FGRPO_F8E4M3 : FGRPO_BF16;
+  b.lens = index_vector(lens, k, "seqused_k");
+  b.cu = index_vector(cu, k, "cu_seqlens", lens.numel() + 1);
+  TORCH_CHECK(table.dim() == 2 && table.size(0) == lens.numel() && table.size(1) < (1LL << 31), "fgrpo: block_table must be [", lens.numel(), ", blocks], got ", table.sizes());
+  TORCH_CHECK(!table.is_floating_point() && table.scalar_type() != at::kBool, "fgrpo: block_table must hold whole numbers, got ", table.scalar_type());
+  require_one_gpu(k, table);
+  b.table = table.to(at::kInt);
+  if (b.table.size(1) > 1 && b.table.stride(1) != 1) b.table = b.table.contiguous();
+  b.B = (int)lens.numel(), b.width = (int)table.size(1);
+  return b;
+}
+
+void paged_cache_write(const Tensor& k_cache, const Tensor& v_cache, const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
+                       const Tensor& k_, const Tensor& v_, const Tensor& table, const Tensor& lens, const Tensor& cu) {
+  no_gradient(k_, "a cache"), no_gradient(v_, "a cache");
+  const PagedBatch b = paged_batch(k_cache, v_cache, k_scale, v_scale, table, lens, cu);
+  require_one_gpu(k_cache, k_, v_);
+  const Tensor k = attn_operand(k_, "k"), v = attn_operand(v_, "v");
+  TORCH_CHECK(k.sizes() == v.sizes() && k.size(1) == k_cache.size(2) && k.size(2) == k_cache.size(3) && k.size(0) < (1LL << 31), "fgrpo: k ", k.sizes(), ", v ", v.sizes(), " do not fit a cache of ", k_cache.sizes());
+  if (k.size(0) == 0 || b.B == 0) return;
+  OnDevice d(k);
+  check(api.fgrpo_paged_cache_write(&b.c, ptr(k), ptr(v), k.stride(0), k.stride(1), v.stride(0), v.stride(1), b.table_ptr(), b.table.stride(0), b.width,
+                                    b.lens.data_ptr<int32_t>(), b.cu.data_ptr<int32_t>(), b.B, (int)k.size(0), d.stream()), "paged_cache_write");
+}
+
+// an output the caller may bring
+Tensor output(const std::optional<Tensor>& given, at::IntArrayRef shape, at::ScalarType type, const Tensor& like, const char* name) {
+  if (!given.has_value()) return at::empty(shape, like.options().dtype(type).requires_grad(false));
+  require_one_gpu(like, *given);
+  TORCH_CHECK(given->sizes() == shape && given->scalar_type() == type && given->is_contiguous() && aligned16(*given), "fgrpo: ", name, " must be ", type, " ", shape, ", contiguous and 16-byte aligned");
+  return *given;
+}
+
+std::vector<Tensor> paged_cache_read(const Tensor& k_cache, const Tensor& v_cache, const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
+                                     const Tensor& table, const Tensor& lens, const Tensor& cu, int64_t total, const std::optional<Tensor>& k_out,
+                                     const std::optional<Tensor>& v_out) {
+  const PagedBatch b = paged_batch(k_cache, v_cache, k_scale, v_scale, table, lens, cu);
+  TORCH_CHECK(total >= 0 && total < (1LL << 31), "fgrpo: total=", total);
+  OnDevice d(k_cache);
+  const Tensor k = output(k_out, {total, b.c.heads, b.c.head_dim}, at::kBFloat16, k_cache, "k_out"), v = output(v_out, {total, b.c.heads, b.c.head_dim}, at::kBFloat16, k_cache, "v_out");
+  if (total > 0 && b.B > 0)
+    check(api.fgrpo_paged_cache_read(&b.c, b.table_ptr(), b.table.stride(0), b.width, b.lens.data_ptr<int32_t>(), b.cu.data_ptr<int32_t>(), b.B, (int)total,
+                                     k.data_ptr(), v.data_ptr(), d.stream()), "paged_cache_read");
+  return {k, v};
+}
+
+std::vector<Tensor> paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const std::optional<Tensor>& k_scale,
+                                    const std::optional<Tensor>& v_scale, const Tensor& table, const Tensor& lens, const Tensor& cu, const std::optional<double>& scale,
+                                    bool causal, int64_t max_len, bool want_lse, const std::optional<Tensor>& out_) {
+  no_gradient(q_, "attention over a cache");
+  const PagedBatch b = paged_batch(k_cache, v_cache, k_scale, v_scale, table, lens, cu);
+  require_one_gpu(k_cache, q_);
+  const Tensor q = attn_operand(q_, "q");
+  TORCH_CHECK(q.size(2) == b.c.head_dim && q.size(1) > 0 && q.size(1) % std::max(b.c.heads, 1) == 0 && q.size(0) < (1LL << 31) && q.size(1) < (1LL << 31),
+              "fgrpo: q ", q.sizes(), " does not fit a cache of ", k_cache.sizes());
+  const int T = (int)q.size(0), Hq = (int)q.size(1);
+  OnDevice d(q);
+  const Tensor out = output(out_, {T, Hq, b.c.head_dim}, at::kBFloat16, q, "out"), lse = want_lse ? at::empty({Hq, T}, q.options().dtype(at::kFloat).requires_grad(false)) : Tensor();
+  if (T > 0 && b.B > 0)
+    check(api.fgrpo_paged_attn_fwd(ptr(q), q.stride(0), q.stride(1), &b.c, b.table_ptr(), b.table.stride(0), b.width, b.lens.data_ptr<int32_t>(),
+                                   b.cu.data_ptr<int32_t>(), b.B, T, Hq, (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(2))), causal,
+                                   out.data_ptr(), want_lse ? fptr(lse) : nullptr, d.stream()), "paged_attn_fwd");
+  return want_lse ? std::vector<Tensor>{out, lse} : std::vector<Tensor>{out};
+}
+
+std::vector<Tensor> verify_drafts(const Tensor& target_, const std::optional<Tensor>& draft_, const Tensor& ids_, const Tensor& u_, const Tensor& cu_) {
+  no_gradient(target_, "verify_drafts");
+  TORCH_CHECK(target_.dim() == 2 && target_.size(0) < (1LL << 31) && target_.size(1) < (1LL << 31), "fgrpo: target must be [tokens, vocabulary], got ", target_.sizes());
+  const int64_t T = target_.size(0), V = target_.size(1);
+  const int code = dtype_code(target_);
+  require_one_gpu(target_, ids_, u_, cu_);
+  const Tensor cu = index_vector(cu_, target_, "cu_seqlens");
+  TORCH_CHECK(cu.numel() >= 1, "fgrpo: cu_seqlens is empty");
+  const int64_t B = cu.numel() - 1;
+  auto rows = [&](const Tensor& t) { return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t.detach() : t.detach().contiguous(); };
+  const Tensor target = rows(target_);
+  Tensor draft = opt(draft_);
+  if (draft.defined()) {
+    no_gradient(draft, "verify_drafts");
+    require_one_gpu(target_, draft);
+    TORCH_CHECK(draft.dim() == 2 && draft.scalar_type() == target.scalar_type() && draft.size(0) <= T && draft.size(1) == V,
+                "fgrpo: draft must be ", target.scalar_type(), " [drafts, ", V, "], got ", draft.scalar_type(), " ", draft.sizes());
+    draft = rows(draft);
+  }
+  TORCH_CHECK(ids_.numel() == T && !ids_.is_floating_point() && u_.numel() == T && u_.is_floating_point(), "fgrpo: ids (whole numbers) and u (floating point) have one entry a row of target");
+  const Tensor ids = ids_.reshape({-1}).to(at::kLong).contiguous(), u = per_token(u_, T, "u");
+  OnDevice d(target);
+  const auto o = target.options().requires_grad(false);
+  Tensor accepted = at::empty({B}, o.dtype(at::kInt)), tokens = at::empty({T}, o.dtype(at::kLong));
+  if (B > 0 && T > 0 && V > 0) {
+    const bool drafts = draft.defined() && draft.size(0) > 0;
+    check(api.fgrpo_verify_drafts(ptr(target), target.stride(0), drafts ? ptr(draft) : nullptr, drafts ? draft.stride(0) : 0, drafts ? (int)draft.size(0) : 0, code, ids.data_ptr<int64_t>(), fptr(u),
+                                  cu.data_ptr<int32_t>(), (int)B, (int)T, (int)V, accepted.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), d.stream()), "verify_drafts");
+  }
+  return {accepted, tokens};
+}
+
 // The numbers of a Python list or tuple into a host array of its length, int64 or float32: what packing a batch spends
 // most of its time on (4 ns an entry; numpy.fromiter 20).  Only plain ints into int64 and plain floats into float32, in their
 // ranges, are taken: false, with the array partly written, for anything else, and numpy's rules decide.
@@ -525,4 +671,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_step", &fused_step, py::call_guard<py::gil_scoped_release>());
   m.def("varlen_attention", &varlen_attention, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu"), py::arg("scale"), py::arg("causal"),
         py::arg("bounds"), py::arg("max_len") = 0, py::call_guard<py::gil_scoped_release>());
+  m.def("paged_cache_write", &paged_cache_write, py::call_guard<py::gil_scoped_release>());
+  m.def("paged_cache_read", &paged_cache_read, py::call_guard<py::gil_scoped_release>());
+  m.def("paged_attention", &paged_attention, py::call_guard<py::gil_scoped_release>());
+  m.def("verify_drafts", &verify_drafts, py::call_guard<py::gil_scoped_release>());
 }

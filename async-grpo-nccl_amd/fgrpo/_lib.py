@@ -11,7 +11,7 @@ from .build import BINDING_PATH, LIB_PATH
 
 ERR = {-1: "bad argument", -2: "unsupported", -3: "workspace", -4: "HIP error", -5: "alignment"}
 
-BF16, F32 = 0, 1
+BF16, F32, F8E4M3 = 0, 1, 2
 AGG_TOKEN_MEAN, AGG_SAMPLE_MEAN = 0, 1
 NUM_STATS = 16
 NUM_PHASES = 5           # FGRPO_NUM_PHASES
@@ -79,7 +79,19 @@ SIGNATURES = {
                                        _vp, _vp, _vp, _i, _vp, _sz, _vp]),
     "fgrpo_varlen_attn_bwd_len": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _ll, _ll, _ll, _ll, _ll, _ll, _vp, _i, _i, _i, _i, _i, _i,
                                        _f, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp, _sz, _vp]),
+    "fgrpo_paged_cache_write": (_i, [_vp, _vp, _vp, _ll, _ll, _ll, _ll, _vp, _ll, _i, _vp, _vp, _i, _i, _vp]),
+    "fgrpo_paged_cache_read": (_i, [_vp, _vp, _ll, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    "fgrpo_paged_attn_fwd": (_i, [_vp, _ll, _ll, _vp, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _f, _i, _vp, _vp, _vp]),
+    "fgrpo_verify_drafts": (_i, [_vp, _ll, _vp, _ll, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
 }
+
+
+class PagedCacheStruct(C.Structure):
+    """``fgrpo_paged_cache`` of the header."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_stride", _ll * 3), ("v_stride", _ll * 3),
+                ("k_scale_stride", _ll * 3), ("v_scale_stride", _ll * 3), ("num_blocks", _i), ("block_size", _i), ("heads", _i),
+                ("head_dim", _i), ("dtype", _i)]
+
 
 _lib = None
 

@@ -23,7 +23,7 @@ _ALT = "" if LIB_PATH == os.path.join(CSRC, "libfgrpo.so") else "_" + os.path.sp
 USAGE_PATH = os.path.join(CSRC, f"resource_usage{_ALT}.json")
 OBJ_DIR = os.path.join(CSRC, "build" + _ALT)
 
-SOURCES = ["fgrpo_api.hip", "launch_lmhead.hip", "launch_gemm.hip", "launch_attn.hip", "launch_attn_keyside.hip"]
+SOURCES = ["fgrpo_api.hip", "launch_lmhead.hip", "launch_gemm.hip", "launch_attn.hip", "launch_attn_keyside.hip", "launch_paged.hip"]
 # This unit keeps its accumulators in named accumulation registers across whole loops.  A clobber list does not reserve
 # them: between two of its statements the compiler may use them, and without this flag it puts the results of the matrix
 # instructions it schedules itself into a[0:15], over the first accumulator, spilling nothing.  The define lets the

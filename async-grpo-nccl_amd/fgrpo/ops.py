@@ -1143,3 +1143,79 @@ def attention_bounds(cu_seqlens: torch.Tensor, T: int, causal: bool = True) -> t
         _lib.check(rc, "varlen_attn_bounds")
     return bounds
 
+
+
+# --------------------------------------------------------------------------- paged cache, the attention over it, drafts
+class PagedCache:
+    """One layer's keys and values in blocks of ``block_size`` tokens: ``k`` / ``v`` [num_blocks, block_size, heads,
+    head_dim] in bf16, or in ``torch.float8_e4m3fn`` with an fp32 scale per (token, head) in ``k_scale`` / ``v_scale``
+    [num_blocks, block_size, heads] (a value is code * scale).  Views are taken as they lie: strides in multiples of 16
+    elements, the innermost dimension contiguous.  ``block_size`` is a power of two from 16 to 65536, ``head_dim`` 128
+    or 64."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                 v_scale: Optional[torch.Tensor] = None):
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @classmethod
+    def empty(cls, num_blocks: int, block_size: int, heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
+              device="cuda") -> "PagedCache":
+        """Room for ``num_blocks * block_size`` tokens.  Nothing is filled: no call reads a place that was not written, as
+        long as the lengths it is given are right."""
+        if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
+            raise RuntimeError(f"fgrpo: a cache is bf16 or float8_e4m3fn, got {dtype}")
+        shape = (int(num_blocks), int(block_size), int(heads), int(head_dim))
+        new = [torch.empty(shape, dtype=dtype, device=device) for _ in range(2)]
+        scales = [torch.empty(shape[:3], dtype=torch.float32, device=device) for _ in range(2)] if dtype != torch.bfloat16 else []
+        return cls(*new, *scales)
+
+
+def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seqused_k: torch.Tensor,
+                      cu_seqlens: torch.Tensor) -> None:
+    """Append new tokens: rows ``cu_seqlens[b]:cu_seqlens[b+1]`` of ``k`` / ``v`` [T, heads, head_dim] bf16 become the last
+    tokens of sequence ``b``, whose length with them is ``seqused_k[b]`` and whose token ``j`` lives in block
+    ``block_table[b, j // block_size]``.  An e4m3 cache is quantised as it is written.  Rows behind the last sequence and
+    positions before a sequence's start go nowhere.  Two rows of one call must not go to one place: what that place then
+    holds is not defined (sequences that share blocks have the shared part written once).  No gradient, no host wait."""
+    _lib.native().paged_cache_write(cache.k, cache.v, cache.k_scale, cache.v_scale, k, v, block_table, seqused_k, cu_seqlens)
+
+
+def paged_cache_read(cache: PagedCache, block_table: torch.Tensor, seqused_k: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                     total: int, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """What the sequences hold, packed: (k, v) [total, heads, head_dim] bf16, the tokens of sequence ``b`` in rows
+    ``cu_seqlens_k[b]:cu_seqlens_k[b+1]`` (``total`` is the last of these).  Rows that no token goes to are left as they are in
+    ``out``, and hold anything without it."""
+    k, v = _lib.native().paged_cache_read(cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, seqused_k, cu_seqlens_k,
+                                          int(total), *(out if out is not None else (None, None)))
+    return k, v
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tensor, seqused_k: torch.Tensor,
+                    cu_seqlens: torch.Tensor, softmax_scale: Optional[float] = None, causal: bool = True, max_len: int = 0,
+                    return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Attention of new tokens over a cache that already holds them: rows ``cu_seqlens[b]:cu_seqlens[b+1]`` of ``q`` [T, Hq, head_dim]
+    bf16 are the last tokens of sequence ``b``, ``seqused_k[b]`` long; token ``i`` of ``n`` sees keys ``j < seqused_k[b]``, and with
+    ``causal`` those with ``j <= seqused_k[b] - n + i``.  Query head ``h`` reads K/V head ``h // (Hq // heads)``.  One token a sequence,
+    drafts, and pieces of prompts may share a call.  Returns [T, Hq, head_dim] bf16, with ``return_lse`` also the log of
+    the softmax denominators, fp32 [Hq, T].  A row that sees nothing gives 0 and -inf; rows behind the last sequence are left as
+    they are in ``out``, and hold anything without it.  ``max_len``: the most new tokens of a sequence, 0 where it is not known:
+    the kernel is chosen by it, results do not depend on it but for the order of fp32 sums.  Values that a query does
+    not see are not read, but for V of keys that other queries of its sequence in the same call see: those must be finite.  No
+    gradient, no host wait."""
+    got = _lib.native().paged_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, seqused_k, cu_seqlens,
+                                        softmax_scale, bool(causal), max_len, bool(return_lse), out)
+    return tuple(got) if return_lse else got[0]
+
+
+def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], ids: torch.Tensor, u: torch.Tensor,
+                  cu_seqlens: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Accept or replace drafted tokens so that what comes out is distributed as ``target``.  Rows ``cu_seqlens[b]:cu_seqlens[b+1]`` are a
+    sequence's last token and its drafts (``ids`` [T]); ``target`` [T, V] the policy's distributions behind each of them; ``draft``
+    [drafts, V] those that the drafts were drawn from, a row for each draft in order (None: drafts that were chosen
+    outright); bf16 or fp32.  ``u`` [T] in [0, 1): row ``i``'s decides on draft ``i``, and the
+    first row whose draft does not stand draws with it.  Returns (how many stand [sequences] int32, tokens [T] int64: those, the
+    one drawn, then -1).  Sums over the vocabulary are held in 64 bits (see ``fgrpo_verify_drafts``)."""
+    accepted, tokens = _lib.native().verify_drafts(target, draft, ids, u, cu_seqlens)
+    return accepted, tokens

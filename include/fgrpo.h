@@ -29,6 +29,7 @@ extern "C" {
 
 #define FGRPO_BF16 0
 #define FGRPO_F32 1
+#define FGRPO_F8E4M3 2 /* paged caches only: e4m3 without infinities, 448 the largest */
 
 #define FGRPO_AGG_TOKEN_MEAN 0
 #define FGRPO_AGG_SAMPLE_MEAN 1
@@ -385,6 +386,61 @@ int fgrpo_varlen_attn_bwd_len(const void* dout, const void* q, const void* k, co
                              int n_seq, int max_len, int T, int Hq, int Hkv, int D, float softmax_scale, int causal, void* dq, void* dk,
                              void* dv, float* delta_ws, int32_t* bounds_ws, int bounds_valid, void* ws, size_t ws_bytes,
                              void* stream);
+
+/* ---- paged key/value cache, and the attention over it --------------------------------
+ * What the policy needs to answer, next to training it: the reference leaves this to its rollout engine
+ * (vllm_worker.py:203-284) and drops flash_attn_varlen_func's block_table (gpu_process_worker.py:265-276).
+ * k / v: [num_blocks][block_size][heads][head_dim] in `dtype` (FGRPO_BF16 or FGRPO_F8E4M3), strides {block, token, head} in
+ * elements, multiples of 16, innermost dimension contiguous, bases 16-byte aligned; k_scale / v_scale (e4m3 only):
+ * fp32 [num_blocks][block_size][heads] with strides of their own.  block_size: a power of two from 16 to 65536; head_dim
+ * 128 or 64.  The struct is read on the host during the call.
+ * The three calls share their description of a batch: block_table [n_seq][width] int32 (rows table_stride entries apart): the
+ * block of a sequence's tokens i*block_size ..; seqused_k [n_seq] int32: a sequence's length, new tokens included;
+ * cu_seqlens [n_seq+1] int32: its rows in the packed arrays.  All on the device, read by the kernels, held inside their arrays
+ * there: cu_seqlens in [0, T], lengths in [0, width*block_size], blocks in [0, num_blocks).
+ * write: row cu[b]+i of k / v [T][heads][head_dim] bf16 (strides in elements, multiples of 8) goes to position
+ * seqused_k[b] - (cu[b+1]-cu[b]) + i of sequence b; rows whose position is negative, and rows behind cu[n_seq], go nowhere.
+ * e4m3: scale = max(max |finite x|, 1e-30) / 448 over a row's head_dim values, code = x * (448 / that max) rounded to nearest even;
+ * infinities and NaN become NaN.  No two rows of a call may go to one place (sequences that share blocks have their shared
+ * part written once): what such a place then holds is not defined.
+ * read: positions 0 .. min(seqused_k[b], cu[b+1]-cu[b])-1 of sequence b to rows cu[b].. of k_out / v_out [total][heads][head_dim]
+ * bf16, contiguous; e4m3: code * scale, rounded.  Other rows are left as they are. */
+typedef struct fgrpo_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  long long k_stride[3], v_stride[3], k_scale_stride[3], v_scale_stride[3];
+  int num_blocks, block_size, heads, head_dim, dtype;
+} fgrpo_paged_cache;
+int fgrpo_paged_cache_write(const fgrpo_paged_cache* cache, const void* k, const void* v, long long k_stride_t, long long k_stride_h,
+                            long long v_stride_t, long long v_stride_h, const int32_t* block_table, long long table_stride, int width,
+                            const int32_t* seqused_k, const int32_t* cu_seqlens, int n_seq, int T, void* stream);
+int fgrpo_paged_cache_read(const fgrpo_paged_cache* cache, const int32_t* block_table, long long table_stride, int width,
+                           const int32_t* seqused_k, const int32_t* cu_seqlens_k, int n_seq, int total, void* k_out, void* v_out,
+                           void* stream);
+/* attention: q [T][Hq][head_dim] bf16 (strides in elements, multiples of 8); row cu[b]+i is token i of the q_b = cu[b+1]-cu[b] last
+ * ones of sequence b and sees its keys j < seqused_k[b], with causal != 0 those with j <= seqused_k[b] - q_b + i.  Query head h reads K/V
+ * head h / (Hq/heads).  out [T][Hq][head_dim] bf16 contiguous; lse [Hq][T] fp32 or NULL (natural log of the softmax
+ * denominator).  A row that sees nothing: out 0, lse -inf.  Rows behind cu[n_seq] are left as they are.  No gradient. */
+int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride_h, const fgrpo_paged_cache* cache,
+                         const int32_t* block_table, long long table_stride, int width, const int32_t* seqused_k,
+                         const int32_t* cu_seqlens_q, int n_seq, int T, int Hq, float softmax_scale, int causal, void* out, float* lse,
+                         void* stream);
+
+/* ---- verification of drafted tokens ---------------------------------------------------
+ * The chunk of sequence b is rows cu[b] .. cu[b+1]-1 of ids [T]: its last token, then K drafted ones.  target [T][V]: row
+ * cu[b]+i is the policy's distribution of what follows the first i+1 of them; draft [draft_rows][V]: a row for each drafted token, in
+ * order: the distribution it was drawn from (NULL: drafts chosen outright, 1 at the token; a row past the end counts as zeros); both `dtype` (bf16 or fp32), rows target_stride /
+ * draft_stride elements apart.  u [T] fp32 in [0, 1).  Draft i, token d, stands while u[cu[b]+i] * draft_i(d) < target_i(d).
+ * accepted[b] = n: how many stand in front of the first that does not.  tokens[cu[b]..]: those n, then one drawn from max(target_n -
+ * draft_n, 0) (where that is all zero, and behind K that stand, from target_n), then -1.  Drawn: the first x
+ * whose running sum over the vocabulary exceeds u[cu[b]+n] times the sum, sums in 64 bits; values that are no probability
+ * (negative, NaN, infinite) count as 0, and a row of zeros gives -1.  tokens behind cu[n_seq] are left as they are; a
+ * sequence without rows has accepted 0.  No counterpart in the reference, whose engine samples by itself. */
+int fgrpo_verify_drafts(const void* target, long long target_stride, const void* draft, long long draft_stride, int draft_rows, int dtype,
+                        const int64_t* ids, const float* u, const int32_t* cu_seqlens, int n_seq, int T, int V, int32_t* accepted,
+                        int64_t* tokens, void* stream);
 
 #ifdef __cplusplus
 }
