@@ -4,7 +4,7 @@
 
 #include "host_common.h"
 #include "draft_kernels.h"
-#include "paged_attn.h"
+#include "paged_rows.h"
 
 using namespace fgrpo;
 
@@ -53,6 +53,35 @@ PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long ta
     HIP_TRY(hipGetLastError());                                                                                        \
   } while (0)
 
+// How a call is divided, from shapes alone.  rb: blocks of 32 rows a wavefront takes (0: work-groups of 128 rows).
+struct RowsPlan {
+  int rb, W;
+};
+RowsPlan plan_rows(const fgrpo_paged_cache* c, int width, int n_seq, int T, int G, int max_len) {
+  const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq;      // not known: the mean
+  RowsPlan r{tokens * G <= 32 ? 1 : tokens * G <= 64 ? 2 : 0, 0};
+  if (r.rb == 0) return r;
+  const long long tiles = (long long)T * G / (32 * r.rb) + n_seq, steps = ((long long)width * c->block_size + 63) / 64 + 1;
+  long long W = 4LL * num_cus();
+  if (tiles * c->heads < W && tiles * c->heads * steps < W) W = tiles * c->heads * steps;
+  r.W = (int)round_up(W, 8);
+  return r;
+}
+size_t rows_bytes(const RowsPlan& r, int D) { return r.rb == 0 ? 0 : 2ull * r.W * (sizeof(int4) + r.rb * 32 * (D * 4 + sizeof(float2))); }
+
+template <int HD, bool FP8, int RB>
+int launch_rows_of(const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
+  hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, RB>), dim3(sp.W), dim3(64), 0, st, p, sp);
+  HIP_TRY(hipGetLastError());
+  hipLaunchKernelGGL((paged_merge_kernel<HD, FP8, RB>), dim3(sp.W, RB * HD / 32), dim3(256), 0, st, p, sp);
+  HIP_TRY(hipGetLastError());
+  return 0;
+}
+template <int HD, bool FP8>
+int launch_rows(int rb, const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
+  return rb == 1 ? launch_rows_of<HD, FP8, 1>(p, sp, st) : launch_rows_of<HD, FP8, 2>(p, sp, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -89,9 +118,14 @@ int fgrpo_paged_cache_read(const fgrpo_paged_cache* cache, const int32_t* block_
   return 0;
 }
 
+size_t fgrpo_paged_attn_workspace(const fgrpo_paged_cache* cache, int width, int n_seq, int T, int Hq, int max_len) {
+  if (!cache || cache->heads <= 0 || Hq <= 0 || Hq % cache->heads || n_seq <= 0 || T <= 0 || width < 0 || (cache->head_dim != 128 && cache->head_dim != 64)) return 0;
+  return rows_bytes(plan_rows(cache, width, n_seq, T, Hq / cache->heads, max_len), cache->head_dim);
+}
+
 int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride_h, const fgrpo_paged_cache* cache, const int32_t* block_table,
                          long long table_stride, int width, const int32_t* seqused_k, const int32_t* cu_seqlens_q, int n_seq, int T, int Hq,
-                         float softmax_scale, int causal, void* out, float* lse, void* stream) {
+                         int max_len, float softmax_scale, int causal, void* out, float* lse, void* ws, size_t ws_bytes, void* stream) {
   const int rc = check_cache("paged_attn_fwd", cache, block_table, table_stride, width, seqused_k, cu_seqlens_q, n_seq, T);
   if (rc) return rc;
   if (!q || !out) return fail(FGRPO_ERR_BAD_ARG, "paged_attn_fwd: null argument");
@@ -100,16 +134,37 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
   if (!aligned16(q) || !aligned16(out)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: q/out must be 16-byte aligned");
   if (q_stride_t < 0 || q_stride_h < 0 || q_stride_t % 8 || q_stride_h % 8)
     return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: strides must be multiples of 8 elements");
+  if (cache->k_stride[1] >= (1LL << 26) || cache->v_stride[1] >= (1LL << 26))      // 16 tokens behind a 32-bit offset
+    return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: tokens of the cache %lld and %lld elements apart", cache->k_stride[1], cache->v_stride[1]);
   const int G = Hq / cache->heads;
   if ((long long)T * G >= (1LL << 31) - 256) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: T=%d rows of %d heads", T, G);
+  hipStream_t st = (hipStream_t)stream;
   PagedAttn p;
   p.c = view_of(cache, block_table, table_stride, width, seqused_k, cu_seqlens_q, n_seq, T);
   p.q = (const bf16_t*)q, p.q_t = q_stride_t, p.q_h = q_stride_h, p.out = (bf16_t*)out, p.lse = lse;
   p.scale = softmax_scale, p.Hq = Hq, p.G = G, p.causal = causal != 0;
-  const long long tiles = ((long long)T * G) / kPagedRows + n_seq;
-  if (cache->heads > 65535 || tiles >= (1LL << 31)) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: %lld tiles of %d heads", tiles, cache->heads);
-  PAGED_DISPATCH(paged_attn_kernel, cache, dim3((unsigned)tiles, cache->heads), 256, (hipStream_t)stream, p);
-  return 0;
+  const RowsPlan plan = plan_rows(cache, width, n_seq, T, G, max_len);
+  if (plan.rb == 0) {
+    const long long tiles = ((long long)T * G) / kPagedRows + n_seq;
+    if (cache->heads > 65535 || tiles >= (1LL << 31)) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: %lld tiles of %d heads", tiles, cache->heads);
+    PAGED_DISPATCH(paged_attn_kernel, cache, dim3((unsigned)tiles, cache->heads), 256, st, p);
+    return 0;
+  }
+  const size_t need = rows_bytes(plan, cache->head_dim);
+  if (!ws || ws_bytes < need) return fail(FGRPO_ERR_WORKSPACE, "paged_attn_fwd: workspace %zu < %zu", ws ? ws_bytes : 0, need);
+  if (!aligned16(ws)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: workspace must be 16-byte aligned");
+  PagedSplit sp;
+  const size_t slots = 2ull * plan.W;
+  sp.W = plan.W;
+  sp.rec = (int4*)ws;
+  sp.part = (float*)((char*)ws + slots * sizeof(int4));
+  sp.ml = (float2*)((char*)sp.part + slots * plan.rb * 32 * cache->head_dim * 4);
+  if (cache->dtype == FGRPO_F8E4M3) {
+    if (cache->head_dim == 128) return launch_rows<128, true>(plan.rb, p, sp, st);
+    return launch_rows<64, true>(plan.rb, p, sp, st);
+  }
+  if (cache->head_dim == 128) return launch_rows<128, false>(plan.rb, p, sp, st);
+  return launch_rows<64, false>(plan.rb, p, sp, st);
 }
 
 int fgrpo_verify_drafts(const void* target, long long target_stride, const void* draft, long long draft_stride, int draft_rows, int dtype,

@@ -48,6 +48,7 @@ struct Api {
   FGRPO_ENTRY(fgrpo_varlen_attn_bwd_len);
   FGRPO_ENTRY(fgrpo_paged_cache_write);
   FGRPO_ENTRY(fgrpo_paged_cache_read);
+  FGRPO_ENTRY(fgrpo_paged_attn_workspace);
   FGRPO_ENTRY(fgrpo_paged_attn_fwd);
   FGRPO_ENTRY(fgrpo_verify_drafts);
 } api;
@@ -82,6 +83,7 @@ void init(const std::unordered_map<std::string, uint64_t>& at) {
   FGRPO_SET(fgrpo_varlen_attn_bwd_len);
   FGRPO_SET(fgrpo_paged_cache_write);
   FGRPO_SET(fgrpo_paged_cache_read);
+  FGRPO_SET(fgrpo_paged_attn_workspace);
   FGRPO_SET(fgrpo_paged_attn_fwd);
   FGRPO_SET(fgrpo_verify_drafts);
 }
@@ -566,10 +568,13 @@ std::vector<Tensor> paged_attention(const Tensor& q_, const Tensor& k_cache, con
   const int T = (int)q.size(0), Hq = (int)q.size(1);
   OnDevice d(q);
   const Tensor out = output(out_, {T, Hq, b.c.head_dim}, at::kBFloat16, q, "out"), lse = want_lse ? at::empty({Hq, T}, q.options().dtype(at::kFloat).requires_grad(false)) : Tensor();
+  const int longest = max_len > 0 && max_len < (1LL << 31) ? (int)max_len : 0;
+  const size_t bytes = T > 0 && b.B > 0 ? api.fgrpo_paged_attn_workspace(&b.c, b.width, b.B, T, Hq, longest) : 0;
+  const Tensor ws = bytes ? workspace(bytes, q) : Tensor();
   if (T > 0 && b.B > 0)
     check(api.fgrpo_paged_attn_fwd(ptr(q), q.stride(0), q.stride(1), &b.c, b.table_ptr(), b.table.stride(0), b.width, b.lens.data_ptr<int32_t>(),
-                                   b.cu.data_ptr<int32_t>(), b.B, T, Hq, (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(2))), causal,
-                                   out.data_ptr(), want_lse ? fptr(lse) : nullptr, d.stream()), "paged_attn_fwd");
+                                   b.cu.data_ptr<int32_t>(), b.B, T, Hq, longest, (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(2))), causal,
+                                   out.data_ptr(), want_lse ? fptr(lse) : nullptr, bytes ? ws.data_ptr() : nullptr, bytes, d.stream()), "paged_attn_fwd");
   return want_lse ? std::vector<Tensor>{out, lse} : std::vector<Tensor>{out};
 }
 

@@ -422,11 +422,15 @@ int fgrpo_paged_cache_read(const fgrpo_paged_cache* cache, const int32_t* block_
 /* attention: q [T][Hq][head_dim] bf16 (strides in elements, multiples of 8); row cu[b]+i is token i of the q_b = cu[b+1]-cu[b] last
  * ones of sequence b and sees its keys j < seqused_k[b], with causal != 0 those with j <= seqused_k[b] - q_b + i.  Query head h reads K/V
  * head h / (Hq/heads).  out [T][Hq][head_dim] bf16 contiguous; lse [Hq][T] fp32 or NULL (natural log of the softmax
- * denominator).  A row that sees nothing: out 0, lse -inf.  Rows behind cu[n_seq] are left as they are.  No gradient. */
+ * denominator).  A row that sees nothing: out 0, lse -inf.  Rows behind cu[n_seq] are left as they are.  No gradient.
+ * max_len: the most rows of a sequence, 0 where it is not known: the kernel and its workspace are chosen by it, results do not depend on it
+ * but for the order of fp32 sums.  ws: 16-byte aligned, fgrpo_paged_attn_workspace bytes for the same arguments (0: may be NULL); nothing in it has
+ * to start at zero, and calls that overlap need one each. */
+size_t fgrpo_paged_attn_workspace(const fgrpo_paged_cache* cache, int width, int n_seq, int T, int Hq, int max_len);
 int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride_h, const fgrpo_paged_cache* cache,
                          const int32_t* block_table, long long table_stride, int width, const int32_t* seqused_k,
-                         const int32_t* cu_seqlens_q, int n_seq, int T, int Hq, float softmax_scale, int causal, void* out, float* lse,
-                         void* stream);
+                         const int32_t* cu_seqlens_q, int n_seq, int T, int Hq, int max_len, float softmax_scale, int causal, void* out,
+                         float* lse, void* ws, size_t ws_bytes, void* stream);
 
 /* ---- verification of drafted tokens ---------------------------------------------------
  * The chunk of sequence b is rows cu[b] .. cu[b+1]-1 of ids [T]: its last token, then K drafted ones.  target [T][V]: row

@@ -47,14 +47,16 @@ def test_caches_are_checked_by_every_call(lib, over, rc):
     assert lib.fgrpo_last_error().startswith(b"paged_attn_fwd: ")
 
 
-def _attend(lib, c, q=AT, q_t=1536, q_h=128, table=AT, table_st=8, width=8, lens=AT, cu=AT, n_seq=2, T=5, Hq=12, scale=0.1, out=AT):
-    return lib.fgrpo_paged_attn_fwd(q, q_t, q_h, c, table, table_st, width, lens, cu, n_seq, T, Hq, scale, 1, out, None, None)
+def _attend(lib, c, q=AT, q_t=1536, q_h=128, table=AT, table_st=8, width=8, lens=AT, cu=AT, n_seq=2, T=5, Hq=12, max_len=0, scale=0.1, out=AT, ws=AT,
+            ws_bytes=1 << 40):
+    return lib.fgrpo_paged_attn_fwd(q, q_t, q_h, c, table, table_st, width, lens, cu, n_seq, T, Hq, max_len, scale, 1, out, None, ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("over,rc", [
     (dict(q=None), -1), (dict(out=None), -1), (dict(lens=None), -1), (dict(cu=None), -1), (dict(table=None), -1), (dict(n_seq=0), -1), (dict(T=0), -1),
     (dict(width=-1), -1), (dict(table_st=4), -1), (dict(width=1 << 27, table_st=1 << 27), -2), (dict(Hq=7), -1), (dict(Hq=0), -1), (dict(scale=0.0), -1),
-    (dict(scale=float("nan")), -1), (dict(q=ODD), -5), (dict(out=ODD), -5), (dict(q_t=100), -5), (dict(q_h=-128), -5)])
+    (dict(scale=float("nan")), -1), (dict(q=ODD), -5), (dict(out=ODD), -5), (dict(q_t=100), -5), (dict(q_h=-128), -5),
+    (dict(ws=None), -3), (dict(ws_bytes=64), -3), (dict(ws=ODD), -5)])
 def test_attention_arguments(lib, over, rc):
     assert _attend(lib, C.byref(_cache()), **over) == rc
     assert lib.fgrpo_last_error().startswith(b"paged_attn_fwd: ")
