@@ -4,11 +4,13 @@
 
 #include "host_common.h"
 #include "draft_kernels.h"
-#include "paged_rows.h"
+#include "paged_tiles.h"
 
 using namespace fgrpo;
 
 namespace {
+
+constexpr long long kMostBetween = 1LL << 26;      // elements between tokens: 16 of them behind a 32-bit offset
 
 int check_cache(const char* who, const fgrpo_paged_cache* c, const int32_t* table, long long table_st, int width, const int32_t* lens,
                 const int32_t* cu, int B, int T) {
@@ -28,6 +30,8 @@ int check_cache(const char* who, const fgrpo_paged_cache* c, const int32_t* tabl
     if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_stride[i] % 16 || c->v_stride[i] % 16)
       return fail(FGRPO_ERR_ALIGN, "%s: strides of the cache must be multiples of 16 elements", who);
     if (fp8 && (c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0)) return fail(FGRPO_ERR_BAD_ARG, "%s: negative stride", who);
+    if (i == 1 && (c->k_stride[i] >= kMostBetween || c->v_stride[i] >= kMostBetween || (fp8 && (c->k_scale_stride[i] >= kMostBetween || c->v_scale_stride[i] >= kMostBetween))))
+      return fail(FGRPO_ERR_UNSUPPORTED, "%s: tokens of the cache 2^26 elements apart or more", who);
   }
   return 0;
 }
@@ -60,26 +64,31 @@ struct RowsPlan {
 RowsPlan plan_rows(const fgrpo_paged_cache* c, int width, int n_seq, int T, int G, int max_len) {
   const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq;      // not known: the mean
   RowsPlan r{tokens * G <= 32 ? 1 : tokens * G <= 64 ? 2 : 0, 0};
-  if (r.rb == 0) return r;
-  const long long tiles = (long long)T * G / (32 * r.rb) + n_seq, steps = ((long long)width * c->block_size + 63) / 64 + 1;
-  long long W = 4LL * num_cus();
+  const long long tiles = (long long)T * G / (r.rb ? 32 * r.rb : kPagedRows) + n_seq, steps = ((long long)width * c->block_size + 63) / 64 + 1;
+  long long W = (r.rb ? 4LL : 2LL) * num_cus();
   if (tiles * c->heads < W && tiles * c->heads * steps < W) W = tiles * c->heads * steps;
   r.W = (int)round_up(W, 8);
   return r;
 }
-size_t rows_bytes(const RowsPlan& r, int D) { return r.rb == 0 ? 0 : 2ull * r.W * (sizeof(int4) + r.rb * 32 * (D * 4 + sizeof(float2))); }
+size_t rows_bytes(const RowsPlan& r, int D) { return 2ull * r.W * (sizeof(int4) + (r.rb ? r.rb : kPagedTileRB) * 32 * (D * 4 + sizeof(float2))); }
 
-template <int HD, bool FP8, int RB>
-int launch_rows_of(const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
-  hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, RB>), dim3(sp.W), dim3(64), 0, st, p, sp);
-  HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL((paged_merge_kernel<HD, FP8, RB>), dim3(sp.W, RB * HD / 32), dim3(256), 0, st, p, sp);
+template <int HD, bool FP8>
+int launch_attn(int rb, const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
+  if (rb == 1) {
+    hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 1>), dim3(sp.W), dim3(64), 0, st, p, sp);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL((paged_merge_kernel<HD, FP8, 1, 1>), dim3(sp.W, HD / 32), dim3(256), 0, st, p, sp);
+  } else if (rb == 2) {
+    hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 2>), dim3(sp.W), dim3(64), 0, st, p, sp);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL((paged_merge_kernel<HD, FP8, 2, 1>), dim3(sp.W, 2 * HD / 32), dim3(256), 0, st, p, sp);
+  } else {
+    hipLaunchKernelGGL((paged_tiles_kernel<HD, FP8>), dim3(sp.W), dim3(256), 0, st, p, sp);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL((paged_merge_kernel<HD, false, kPagedTileRB, HD / 32>), dim3(2 * sp.W, kPagedTileRB), dim3(256), 0, st, p, sp);
+  }
   HIP_TRY(hipGetLastError());
   return 0;
-}
-template <int HD, bool FP8>
-int launch_rows(int rb, const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
-  return rb == 1 ? launch_rows_of<HD, FP8, 1>(p, sp, st) : launch_rows_of<HD, FP8, 2>(p, sp, st);
 }
 
 }  // namespace
@@ -134,8 +143,6 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
   if (!aligned16(q) || !aligned16(out)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: q/out must be 16-byte aligned");
   if (q_stride_t < 0 || q_stride_h < 0 || q_stride_t % 8 || q_stride_h % 8)
     return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: strides must be multiples of 8 elements");
-  if (cache->k_stride[1] >= (1LL << 26) || cache->v_stride[1] >= (1LL << 26))      // 16 tokens behind a 32-bit offset
-    return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: tokens of the cache %lld and %lld elements apart", cache->k_stride[1], cache->v_stride[1]);
   const int G = Hq / cache->heads;
   if ((long long)T * G >= (1LL << 31) - 256) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: T=%d rows of %d heads", T, G);
   hipStream_t st = (hipStream_t)stream;
@@ -144,27 +151,21 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
   p.q = (const bf16_t*)q, p.q_t = q_stride_t, p.q_h = q_stride_h, p.out = (bf16_t*)out, p.lse = lse;
   p.scale = softmax_scale, p.Hq = Hq, p.G = G, p.causal = causal != 0;
   const RowsPlan plan = plan_rows(cache, width, n_seq, T, G, max_len);
-  if (plan.rb == 0) {
-    const long long tiles = ((long long)T * G) / kPagedRows + n_seq;
-    if (cache->heads > 65535 || tiles >= (1LL << 31)) return fail(FGRPO_ERR_UNSUPPORTED, "paged_attn_fwd: %lld tiles of %d heads", tiles, cache->heads);
-    PAGED_DISPATCH(paged_attn_kernel, cache, dim3((unsigned)tiles, cache->heads), 256, st, p);
-    return 0;
-  }
   const size_t need = rows_bytes(plan, cache->head_dim);
   if (!ws || ws_bytes < need) return fail(FGRPO_ERR_WORKSPACE, "paged_attn_fwd: workspace %zu < %zu", ws ? ws_bytes : 0, need);
   if (!aligned16(ws)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: workspace must be 16-byte aligned");
   PagedSplit sp;
   const size_t slots = 2ull * plan.W;
-  sp.W = plan.W;
+  sp.W = plan.W, sp.odd = plan.rb != 0;
   sp.rec = (int4*)ws;
   sp.part = (float*)((char*)ws + slots * sizeof(int4));
-  sp.ml = (float2*)((char*)sp.part + slots * plan.rb * 32 * cache->head_dim * 4);
+  sp.ml = (float2*)((char*)sp.part + slots * (plan.rb ? plan.rb : kPagedTileRB) * 32 * cache->head_dim * 4);
   if (cache->dtype == FGRPO_F8E4M3) {
-    if (cache->head_dim == 128) return launch_rows<128, true>(plan.rb, p, sp, st);
-    return launch_rows<64, true>(plan.rb, p, sp, st);
+    if (cache->head_dim == 128) return launch_attn<128, true>(plan.rb, p, sp, st);
+    return launch_attn<64, true>(plan.rb, p, sp, st);
   }
-  if (cache->head_dim == 128) return launch_rows<128, false>(plan.rb, p, sp, st);
-  return launch_rows<64, false>(plan.rb, p, sp, st);
+  if (cache->head_dim == 128) return launch_attn<128, false>(plan.rb, p, sp, st);
+  return launch_attn<64, false>(plan.rb, p, sp, st);
 }
 
 int fgrpo_verify_drafts(const void* target, long long target_stride, const void* draft, long long draft_stride, int draft_rows, int dtype,

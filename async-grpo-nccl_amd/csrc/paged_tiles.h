@@ -1,0 +1,362 @@
+// Attention over a paged cache for many rows a sequence (pieces of prompts, scored answers): bound by the matrix instructions and the
+// vector arithmetic beside them.  (What is computed: paged_attn.h; how it is dealt out: paged_deal.h.)
+//
+// A work-group of four wavefronts has 128 rows of a sequence and K/V head, 32 a wavefront, and walks their keys 64 at a time through two
+// LDS buffers, with one barrier a step and the fragment schedule of varlen_attn_fwd2_kernel (attn_kernels.h): two
+// work-groups a CU, so that one wavefront's softmax runs beside another's matrix instructions.  Wavefront w fetches keys 16 w .. of
+// a step, which lie in one page: one look-up by the scalar unit, a step ahead.
+// bf16 travels global -> LDS directly.  e4m3 is converted once for the four wavefronts: codes wait in registers for a step (16 of them), and
+// are written to LDS as bf16, which holds them exactly; the scales of a step's keys lie beside the tiles in LDS.
+//
+// Dealing out: a launch of W work-groups, all resident.  Where the heaviest item is more than two mean shares, or there are fewer items than
+// work-groups, shares of the weights, cut inside items (a cut costs 64 KiB of sums written and read per part).  Else whole items, W / 8 a round for
+// the W / 8 work-groups of an XCD, alternately from either end (under the causal mask weights ascend); what is left for the last
+// round is cut into as many parts as make it shortest.
+#pragma once
+#include "paged_rows.h"
+
+namespace fgrpo {
+
+constexpr int kPagedTileRB = kPagedRows / 32;
+
+template <int HD, bool FP8>
+struct PagedTiles {
+  static constexpr int ES = FP8 ? 1 : 2, RBY = HD * ES, TILE = kAttnBK * HD * 2, BUF = 2 * TILE;
+  static constexpr int CPR = RBY / 16, RPI = 1024 / RBY, IPG = 16 / RPI;      // as the cache has its rows: 16-byte chunks, rows and instructions of 16 keys
+  static constexpr int T0 = FP8 ? 4 * kAttnBK * 4 : 0, LDS = T0 + 2 * BUF;      // the scales of both buffers lie in front (K, then V)
+};
+
+// Parts of the last, incomplete round of `left` items on `n` work-groups: the shortest of rounds / parts, a cut costing about a 20th of an item.
+__device__ __forceinline__ int paged_last_parts(int left, int n) {
+  int best = 1;
+  float cost = (float)((left + n - 1) / n);
+  for (int parts = 2; parts <= 8 && left * parts <= 2 * n; ++parts) {
+    const float c = (float)((left * parts + n - 1) / n) / parts + 0.05f * parts;
+    if (c < cost) cost = c, best = parts;
+  }
+  return best;
+}
+
+template <int HD, bool FP8>
+static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p, PagedSplit sp) {
+  using C = PagedTiles<HD, FP8>;
+  constexpr int KS = HD / 16, DB = HD / 32, G4 = KS / 2, ROWS = kPagedRows;
+  __shared__ __attribute__((aligned(16))) char smem[C::LDS];
+  const uint32_t lds0 = lds_addr(smem);
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int xcd = blockIdx.x & 7, n = sp.W >> 3, me = blockIdx.x >> 3, w = xcd * n + me;
+  // fragment addresses: of k step st the row's first with bits of its chunk flipped, of column block db likewise (AttnLane)
+  uint32_t row_at, tr_at[2];
+  {
+    const AttnLane<HD> L = attn_lane<HD>(lane);
+    row_at = L.rowc[0] + lds0 + C::T0, tr_at[0] = L.tr[0][0] + lds0 + C::T0, tr_at[1] = L.tr[0][1] + lds0 + C::T0;
+  }
+  auto anew = [](uint32_t x) {      // formed at each use: e4m3 has no registers to carry all of them
+    if constexpr (FP8) asm volatile("" : "+v"(x));
+    return x;
+  };
+  const float c = p.scale * kLog2e;
+  // where this wavefront's lanes read: row lane / CPR of 16 and every RPI-th behind it, and of instruction i chunk `ch`, but for the bits of
+  // the swizzle that i decides; and, codes, where they write (of 16 codes the first eight; the others and other i flip bits)
+  const int row16 = lane / C::CPR, at16 = 16 * wave + row16, ch = FP8 ? lane % C::CPR : (lane % C::CPR) ^ attn_swz<HD>(at16);
+  const uint32_t voff_k = (uint32_t)(row16 * p.c.k_st[1] * C::ES), voff_v = (uint32_t)(row16 * p.c.v_st[1] * C::ES);
+  const uint32_t put = lds0 + C::T0 + at16 * (HD * 2) + (((2 * ch) ^ attn_swz<HD>(at16)) << 4);
+  auto flip = [](int i) { return attn_swz<HD>(i * C::RPI); };      // the swizzle of row16 + i RPI is that of row16 with these bits flipped: RPI is a power of two above row16
+
+  // x0 .. x1 of an item's weight; whole: its output, else sums for `slot`
+  auto walk = [&](const PagedItem& s, const PagedWeight& wt, double x0, double x1, int slot) {
+    const double weight = wt.of(s.t);
+    const bool whole = x0 <= 0 && x1 >= weight;
+    const int q0 = __builtin_amdgcn_readfirstlane(wt.q0), nq = __builtin_amdgcn_readfirstlane(wt.nq), len = __builtin_amdgcn_readfirstlane(wt.len);
+    const int rows = nq * p.G, r0 = s.t * ROWS, rw = r0 + 32 * wave;
+    const int k_end = __builtin_amdgcn_readfirstlane(paged_sight(p, wt, r0, ROWS).most);
+    const PagedRange kr = paged_range<kAttnBK>(x0, x1, weight, k_end);
+    const int k0 = kr.k0, k1 = kr.k1;
+    const bool wave_on = rw < rows;
+    const PagedSight sight = paged_sight(p, wt, wave_on ? rw : r0, 32);
+    const int w_most = wave_on ? __builtin_amdgcn_readfirstlane(sight.most) : 0, w_least = __builtin_amdgcn_readfirstlane(sight.least);
+
+    int page = 0;
+    auto look_up = [&](int kb) { page = paged_table_at(p.c, s.b, (kb + 16 * wave) >> p.c.page_log2); };
+    u32x4_t raw[FP8 ? 2 * C::IPG : 1];
+    uint32_t raw_scale[2] = {0u, 0u};
+    // tile kb: into LDS (bf16), or into registers
+    auto fetch = [&](int buf, int kb) {
+      page = min(max(page, 0), p.c.num_pages - 1);
+      const int j = kb + 16 * wave, place = j & ((1 << p.c.page_log2) - 1), m = min(max(k_end - j, 0), 16);
+      const __amdgpu_buffer_rsrc_t rk = make_rsrc(p.c.k + paged_offset(p.c.k_st, page, place, s.head) * C::ES, m ? (uint32_t)((m - 1) * p.c.k_st[1] * C::ES) + C::RBY : 0);
+      const __amdgpu_buffer_rsrc_t rv = make_rsrc(p.c.v + paged_offset(p.c.v_st, page, place, s.head) * C::ES, m ? (uint32_t)((m - 1) * p.c.v_st[1] * C::ES) + C::RBY : 0);
+      if constexpr (FP8) {
+        const __amdgpu_buffer_rsrc_t sk = make_rsrc(p.c.k_scale + paged_offset(p.c.ks_st, page, place, s.head), m ? (uint32_t)((m - 1) * p.c.ks_st[1] * 4) + 4 : 0);
+        const __amdgpu_buffer_rsrc_t sv = make_rsrc(p.c.v_scale + paged_offset(p.c.vs_st, page, place, s.head), m ? (uint32_t)((m - 1) * p.c.vs_st[1] * 4) + 4 : 0);
+        raw_scale[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_raw_buffer_load_b32(sk, (int)((lane & 15) * (uint32_t)p.c.ks_st[1] * 4), 0, 0));
+        raw_scale[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_raw_buffer_load_b32(sv, (int)((lane & 15) * (uint32_t)p.c.vs_st[1] * 4), 0, 0));
+#pragma unroll
+        for (int i = 0; i < C::IPG; ++i) {
+          raw[2 * i] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)(voff_k + ch * 16), (int)(i * C::RPI * p.c.k_st[1]), 0));
+          raw[2 * i + 1] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, (int)(voff_v + ch * 16), (int)(i * C::RPI * p.c.v_st[1]), 0));
+        }
+      } else {
+        char* t = smem + buf * C::BUF + wave * (16 * C::RBY);
+#pragma unroll
+        for (int i = 0; i < C::IPG; ++i) {
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, FGRPO_LDS_PTR(t + i * 1024), 16, (int)(voff_k + (ch ^ flip(i)) * 16), (int)(i * C::RPI * p.c.k_st[1] * 2), 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, FGRPO_LDS_PTR(t + C::TILE + i * 1024), 16, (int)(voff_v + (ch ^ flip(i)) * 16), (int)(i * C::RPI * p.c.v_st[1] * 2), 0, 0);
+        }
+      }
+      look_up(kb + kAttnBK);
+    };
+    auto put_codes = [&](auto bufc) {      // registers -> LDS, as bf16
+      constexpr int buf = decltype(bufc)::value;
+      if constexpr (FP8) {
+#pragma unroll
+        for (int i = 0; i < C::IPG; ++i)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t at = (put ^ ((u ^ flip(i)) << 4)) + i * C::RPI * (HD * 2);
+            lds_write_u128_asm<buf * C::BUF>(at, paged_codes_to_bf16(raw[2 * i][2 * u], raw[2 * i][2 * u + 1]));
+            lds_write_u128_asm<buf * C::BUF + C::TILE>(at, paged_codes_to_bf16(raw[2 * i + 1][2 * u], raw[2 * i + 1][2 * u + 1]));
+          }
+        if (lane < 16) {
+          lds_write_u32_asm<buf * 2 * kAttnBK * 4>(lds0 + (16 * wave + lane) * 4, raw_scale[0]);
+          lds_write_u32_asm<buf * 2 * kAttnBK * 4 + kAttnBK * 4>(lds0 + (16 * wave + lane) * 4, raw_scale[1]);
+        }
+      }
+    };
+    using I0 = std::integral_constant<int, 0>;
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+
+    const int row = rw + (lane & 31), tok = row / p.G, hq = s.head * p.G + row % p.G;
+    const bool valid = row < rows;
+    const int seen = !valid || !p.causal ? k_end : min(max(len - nq + tok + 1, 0), len);
+    if (k0 < k1) {
+      look_up(k0);
+      fetch(0, k0);
+    }
+    bf16x8_t qf[KS];
+    attn_row_operand(qf, p.q + (long long)(q0 + (valid ? tok : 0)) * p.q_t + (long long)hq * p.q_h, valid, h);
+    f32x16_t acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;      // the maximum in powers of two
+    bool started = false;
+    if constexpr (FP8) {
+      if (k0 < k1) put_codes(I0{});
+      if (k0 + kAttnBK < k1) fetch(0, k0 + kAttnBK);
+      wait_lgkm<0>();
+    } else {
+      FGRPO_WAIT_VMCNT(0);
+    }
+    wg_barrier();
+    auto step = [&](auto curc, int kb) {
+      constexpr int cur = decltype(curc)::value, kt = cur * C::BUF, vt = kt + C::TILE;
+      if (kb + kAttnBK < k1) {
+        if constexpr (FP8) {
+          put_codes(std::integral_constant<int, cur ^ 1>{});
+          if (kb + 2 * kAttnBK < k1) fetch(0, kb + 2 * kAttnBK);
+        } else {
+          fetch(cur ^ 1, kb + kAttnBK);
+        }
+      }
+      if (kb < w_most) {
+        u32x4_t kf[2][G4];
+        AttnTr vq[2][DB];
+        f32x16_t s2[2];
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s2[mb][r] = 0.f;
+        auto req_k = [&](auto gc) {
+          constexpr int g = decltype(gc)::value;
+          const uint32_t at = anew(row_at);
+          static_for<G4>([&](auto ic) {
+            constexpr int i = decltype(ic)::value, st = G4 * (g % 2) + i;
+            kf[g % 2][i] = lds_read_u128_asm<kt + (g / 2) * 32 * HD * 2>(at ^ (st << 5));
+          });
+        };
+        auto req_v = [&](auto qc) {
+          constexpr int q = decltype(qc)::value;
+          const uint32_t lo = anew(tr_at[0]), hi = anew(tr_at[1]);
+          static_for<DB>([&](auto dc) {
+            constexpr int db = decltype(dc)::value;
+            vq[q % 2][db] = attn_rd_tr_asm<vt + 16 * q * HD * 2>(lo ^ (db << 6), hi ^ (db << 6));
+          });
+        };
+        auto mma_k = [&](auto gc) {
+          constexpr int g = decltype(gc)::value;
+#pragma unroll
+          for (int i = 0; i < G4; ++i) {
+            attn_settle(kf[g % 2][i]);
+            s2[g / 2] = attn_mfma(kf[g % 2][i], __builtin_bit_cast(u32x4_t, qf[G4 * (g % 2) + i]), s2[g / 2]);
+          }
+        };
+        // scales of the 32 keys of a half, four instructions' worth
+        auto scale_by = [&](auto mbc, auto which) {
+          constexpr int mb = decltype(mbc)::value;
+          u32x4_t f[4];
+          paged_read_scales<cur * 2 * kAttnBK * 4 + decltype(which)::value * kAttnBK * 4 + mb * 128>(f, lds0 + 16 * h);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s2[mb][r] *= __uint_as_float(f[r >> 2][r & 3]);
+        };
+        req_k(I0{});
+        req_k(I1{});
+        wait_lgkm<G4>();
+        __builtin_amdgcn_sched_barrier(0);
+        mma_k(I0{});
+        __builtin_amdgcn_sched_barrier(0);
+        req_k(I2{});
+        wait_lgkm<G4>();
+        __builtin_amdgcn_sched_barrier(0);
+        mma_k(I1{});
+        __builtin_amdgcn_sched_barrier(0);
+        req_k(I3{});
+        req_v(I0{});
+        wait_lgkm<G4 + 2 * DB>();
+        __builtin_amdgcn_sched_barrier(0);
+        mma_k(I2{});
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lgkm<2 * DB>();
+        __builtin_amdgcn_sched_barrier(0);
+        mma_k(I3{});
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (FP8) scale_by(I0{}, I0{}), scale_by(I1{}, I0{});
+        float mx = -INFINITY;
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          if (kb + 32 * mb + 32 > w_least) {
+            const int at = kb + 32 * mb + 4 * h;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s2[mb][r] = at + 8 * (r >> 2) + (r & 3) < seen ? s2[mb][r] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s2[mb][r]);
+        {
+          float mlo, mhi;
+          attn_halves(mx, mlo, mhi);
+          mx = fmaxf(mlo, mhi);
+        }
+        const float m_new = fmaxf(m_run, mx * c), m_use = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m_run - m_use);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float e = fast_exp2(__builtin_fmaf(s2[mb][r], c, -m_use));
+            s2[mb][r] = e;
+            sum[mb] += e;
+          }
+        l_run = l_run * alpha + (sum[0] + sum[1]);
+        m_run = m_new;
+        if (started && __any(alpha != 1.f)) {
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+        }
+        if constexpr (FP8) scale_by(I0{}, I1{}), scale_by(I1{}, I1{});
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<4>([&](auto qc) {
+          constexpr int q = decltype(qc)::value, mb = q / 2, half = q % 2;
+          if constexpr (q < 3) req_v(std::integral_constant<int, q + 1>{});
+          wait_lgkm<(q < 3 ? 2 * DB : 0)>();
+          __builtin_amdgcn_sched_barrier(0);
+          float tmp[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) tmp[j] = s2[mb][8 * half + j];
+          const u32x4_t pf = __builtin_bit_cast(u32x4_t, attn_pack8(tmp));
+#pragma unroll
+          for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(attn_settle_tr(vq[q % 2][db]), pf, acc[db]);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        started = true;
+      }
+      if constexpr (!FP8) FGRPO_WAIT_VMCNT(0);
+      wait_lgkm<0>();
+      wg_barrier();
+    };
+    for (int kb = k0; kb < k1; kb += 2 * kAttnBK) {
+      step(I0{}, kb);
+      if (kb + kAttnBK < k1) step(I1{}, kb + kAttnBK);
+    }
+    float l_lo, l_hi;
+    attn_halves(l_run, l_lo, l_hi);
+    const float l = l_lo + l_hi;
+    int lane_e = lane;
+    asm volatile("" : "+v"(lane_e));      // the row's addresses formed anew: held across the loop, they would cost registers
+    const int row_e = rw + (lane_e & 31), tok_e = q0 + row_e / p.G, hq_e = s.head * p.G + row_e % p.G;
+    if (row_e >= rows) return;
+    if (whole) {
+      attn_store_rowmajor(acc, l > 0.f ? 1.f / l : 0.f, p.out + ((long long)tok_e * p.Hq + hq_e) * HD, h);
+      if (p.lse && h == 0) p.lse[(long long)hq_e * p.c.T + tok_e] = paged_lse(m_run, l);
+    } else {
+      attn_store_partial(acc, sp.part + ((long long)slot * kPagedTileRB + wave) * (32 * HD), lane_e);
+      if (h == 0) sp.ml[((long long)slot * kPagedTileRB + wave) * 32 + lane_e] = make_float2(m_run, l);
+    }
+  };
+
+  const PagedTotal total = paged_total<ROWS>(p);
+  const int4 none = make_int4(0, 0, 0, 0);
+  const bool shares = total.items < sp.W || total.most * sp.W > 2 * total.weight;
+  const PagedShares sh = paged_shares(total, sp.W, 2.0 * kAttnBK * p.G);
+  double done = 0, hi = 0;                                    // shares: this one
+  int first = 0, rounds = 0, left = 0, parts = 1, turn = 0;      // whole items: the XCD's first, rounds of n, those of the last round, their parts; this work-group's turn
+  PagedItem s{0, 0, 0, 0, 0};
+  if (shares) {
+    if (threadIdx.x == 0) sp.rec[2 * w] = sp.rec[2 * w + 1] = none;
+    if (!(w < sh.used)) return;
+    done = sh.bound(w), hi = sh.bound(w + 1);
+    if (!(done < hi)) return;
+    s = paged_item<ROWS, false>(p, done);
+  } else {                       // those that begin in this XCD's eighth of the weights
+    if (threadIdx.x == 0) sp.rec[2 * n * xcd + me] = sp.rec[2 * n * xcd + n + me] = none;
+    first = __builtin_amdgcn_readfirstlane((int)paged_item<ROWS, false>(p, floor(total.weight * xcd / 8)).index);
+    const int last = xcd == 7 ? (int)total.items : (int)paged_item<ROWS, false>(p, floor(total.weight * (xcd + 1) / 8)).index;
+    const int items = __builtin_amdgcn_readfirstlane(last) - first;
+    rounds = items / n, left = items - rounds * n, parts = __builtin_amdgcn_readfirstlane(paged_last_parts(left, n));
+  }
+  for (;;) {
+    double x0 = 0, x1;
+    int slot = 0, part = 0;
+    if (!shares) {
+      if (turn < rounds) {
+        s = paged_item<ROWS, true>(p, first + turn * n + (turn & 1 ? n - 1 - me : me));
+      } else {
+        const int i = (turn - rounds) * n + me;
+        if (i >= left * parts || turn - rounds > 1) break;
+        s = paged_item<ROWS, true>(p, first + rounds * n + i / parts);
+        slot = 2 * n * xcd + i, part = i % parts;
+      }
+      ++turn;
+    }
+    if (s.b >= p.c.B) break;
+    const PagedWeight wt = paged_weight<ROWS>(p, s.b);
+    const double weight = wt.of(s.t);
+    int4 rec = none;
+    if (shares) {
+      x0 = done - s.at, x1 = fmin(hi - s.at, weight);
+      slot = 2 * w + (x0 <= 0);
+      if (x0 <= 0 && x1 < weight) rec = make_int4(s.b + 1, s.t, s.head, sh.holding(s.at + weight - 1) - w + 1);
+    } else if (turn > rounds) {
+      x0 = floor(weight * part / parts), x1 = floor(weight * (part + 1) / parts);
+      if (parts > 1 && part == 0) rec = make_int4(s.b + 1, s.t, s.head, -parts);
+    } else {
+      x1 = weight;
+    }
+    if (rec.x != 0 && threadIdx.x == 0) sp.rec[slot] = rec;
+    walk(s, wt, x0, x1, slot);
+    if (shares) {
+      paged_next<ROWS>(p, s, paged_weight<ROWS>(p, s.b));
+      done = s.at;
+      if (!(done < hi)) break;
+    }
+  }
+}
+
+}  // namespace fgrpo

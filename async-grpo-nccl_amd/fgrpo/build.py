@@ -54,6 +54,8 @@ TWO_PER_SIMD = ("TileCfgILi256ELi256ELi64ELi2ELi4ELi2ELi2ELb1EE",      # id 8
                 "varlen_attn_fwd2_kernel", "varlen_attn_dq2_kernel", "varlen_attn_dkv2_kernel")
 # attention kernels whose LDS reads are inline assembly: a spilled register could be one whose data is still on its way
 ASM_READ_ATTN = ("varlen_attn_fwd2_kernel", "varlen_attn_dq2_kernel", "varlen_attn_dkv2_kernel")
+# ... the paged attention's tiles are no different (its kernel for few rows waits inside its assembly)
+ASM_READ_PAGED = ("paged_tiles_kernel",)
 # ... and the one with named accumulation registers (head dimension x key blocks of them): no spills either, and exactly
 # those; with one key block it runs two wavefronts per SIMD
 ASM_READ_NAMED_ACC = ("varlen_attn_dkv3_kernel",)
@@ -94,7 +96,7 @@ def check_resource_usage(usage: dict) -> list:
         if tile and ASM_READ_CFG.search(name) and (u.get("scratch", 0) or u.get("vgpr_spill", 0)):
             bad.append(f"{name}: inline-assembly fragment reads with {u.get('vgpr_spill')} spilled VGPRs "
                        f"({u.get('scratch')} B/lane of scratch)")
-        if any(k in name for k in ASM_READ_ATTN + ASM_READ_NAMED_ACC) and (u.get("scratch", 0) or u.get("vgpr_spill", 0)):
+        if any(k in name for k in ASM_READ_ATTN + ASM_READ_PAGED + ASM_READ_NAMED_ACC) and (u.get("scratch", 0) or u.get("vgpr_spill", 0)):
             bad.append(f"{name}: inline-assembly fragment reads with {u.get('vgpr_spill')} spilled VGPRs "
                        f"({u.get('scratch')} B/lane of scratch)")
         if any(k in name for k in TWO_PER_SIMD) and (tile or "varlen" in name):
