@@ -91,6 +91,18 @@ int launch_attn(int rb, const PagedAttn& p, const PagedSplit& sp, hipStream_t st
   return 0;
 }
 
+int verify_chunks(int V) { return (V + kVerifyChunk - 1) / kVerifyChunk; }
+size_t verify_sums_bytes(int n_seq, int V) { return (size_t)n_seq * verify_chunks(V) * sizeof(double2); }
+
+template <bool F32, bool ALIGNED>
+int launch_verify(const VerifyParams& p, hipStream_t st) {
+  hipLaunchKernelGGL((verify_sums_kernel<F32, ALIGNED>), dim3(p.B * p.chunks), dim3(kVerifyThreads), 0, st, p);
+  HIP_TRY(hipGetLastError());
+  hipLaunchKernelGGL((verify_draw_kernel<F32, ALIGNED>), dim3(p.B), dim3(kVerifyThreads), 0, st, p);
+  HIP_TRY(hipGetLastError());
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -168,17 +180,31 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
   return launch_attn<64, false>(plan.rb, p, sp, st);
 }
 
+size_t fgrpo_verify_drafts_workspace(int n_seq, int V) {
+  if (n_seq <= 0 || V <= 0) return 0;
+  return verify_sums_bytes(n_seq, V) + (size_t)n_seq * sizeof(int);
+}
+
 int fgrpo_verify_drafts(const void* target, long long target_stride, const void* draft, long long draft_stride, int draft_rows, int dtype,
                         const int64_t* ids, const float* u, const int32_t* cu_seqlens, int n_seq, int T, int V, int32_t* accepted, int64_t* tokens,
-                        void* stream) {
+                        void* ws, size_t ws_bytes, void* stream) {
   if (!target || !ids || !u || !cu_seqlens || !accepted || !tokens) return fail(FGRPO_ERR_BAD_ARG, "verify_drafts: null argument");
   if (n_seq <= 0 || T <= 0 || V <= 0 || target_stride < V || draft_rows < 0 || (draft && draft_stride < V))
     return fail(FGRPO_ERR_BAD_ARG, "verify_drafts: n_seq=%d T=%d V=%d, rows %lld and %lld apart", n_seq, T, V, target_stride, draft_stride);
   if (dtype != FGRPO_BF16 && dtype != FGRPO_F32) return fail(FGRPO_ERR_BAD_ARG, "verify_drafts: dtype=%d", dtype);
-  VerifyParams p{target, draft, (const long long*)ids, u, cu_seqlens, target_stride, draft_stride, n_seq, T, V, dtype == FGRPO_F32, draft_rows, accepted, (long long*)tokens};
-  hipLaunchKernelGGL(verify_drafts_kernel, dim3(n_seq), dim3(1024), 0, (hipStream_t)stream, p);
-  HIP_TRY(hipGetLastError());
-  return 0;
+  if (V > 0x7fffffff - 2 * kVerifyChunk || (long long)n_seq * verify_chunks(V) >= (1LL << 31))
+    return fail(FGRPO_ERR_UNSUPPORTED, "verify_drafts: %d sequences over a vocabulary of %d", n_seq, V);
+  const size_t need = fgrpo_verify_drafts_workspace(n_seq, V);
+  if (!ws || ws_bytes < need) return fail(FGRPO_ERR_WORKSPACE, "verify_drafts: workspace %zu < %zu", ws ? ws_bytes : 0, need);
+  if (!aligned16(ws)) return fail(FGRPO_ERR_ALIGN, "verify_drafts: workspace must be 16-byte aligned");
+  VerifyParams p{target, draft, (const long long*)ids, u, cu_seqlens, target_stride, draft_stride, n_seq, T, V, draft_rows, verify_chunks(V), accepted, (long long*)tokens,
+                 (double2*)ws, (int*)((char*)ws + verify_sums_bytes(n_seq, V))};
+  const bool f32 = dtype == FGRPO_F32;
+  const long long es = f32 ? 4 : 2;      // rows that begin at multiples of 16 bytes are read 16 bytes at a time: half the time of a vocabulary of 32000, where loads are in short supply
+  const bool whole = aligned16(target) && target_stride * es % 16 == 0 && (!draft || (aligned16(draft) && draft_stride * es % 16 == 0));
+  hipStream_t st = (hipStream_t)stream;
+  if (f32) return whole ? launch_verify<true, true>(p, st) : launch_verify<true, false>(p, st);
+  return whole ? launch_verify<false, true>(p, st) : launch_verify<false, false>(p, st);
 }
 
 }  // extern "C"

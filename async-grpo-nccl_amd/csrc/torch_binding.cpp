@@ -50,6 +50,7 @@ struct Api {
   FGRPO_ENTRY(fgrpo_paged_cache_read);
   FGRPO_ENTRY(fgrpo_paged_attn_workspace);
   FGRPO_ENTRY(fgrpo_paged_attn_fwd);
+  FGRPO_ENTRY(fgrpo_verify_drafts_workspace);
   FGRPO_ENTRY(fgrpo_verify_drafts);
 } api;
 
@@ -85,6 +86,7 @@ void init(const std::unordered_map<std::string, uint64_t>& at) {
   FGRPO_SET(fgrpo_paged_cache_read);
   FGRPO_SET(fgrpo_paged_attn_workspace);
   FGRPO_SET(fgrpo_paged_attn_fwd);
+  FGRPO_SET(fgrpo_verify_drafts_workspace);
   FGRPO_SET(fgrpo_verify_drafts);
 }
 
@@ -604,8 +606,9 @@ std::vector<Tensor> verify_drafts(const Tensor& target_, const std::optional<Ten
   Tensor accepted = at::empty({B}, o.dtype(at::kInt)), tokens = at::empty({T}, o.dtype(at::kLong));
   if (B > 0 && T > 0 && V > 0) {
     const bool drafts = draft.defined() && draft.size(0) > 0;
+    const Tensor ws = workspace(api.fgrpo_verify_drafts_workspace((int)B, (int)V), target);
     check(api.fgrpo_verify_drafts(ptr(target), target.stride(0), drafts ? ptr(draft) : nullptr, drafts ? draft.stride(0) : 0, drafts ? (int)draft.size(0) : 0, code, ids.data_ptr<int64_t>(), fptr(u),
-                                  cu.data_ptr<int32_t>(), (int)B, (int)T, (int)V, accepted.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), d.stream()), "verify_drafts");
+                                  cu.data_ptr<int32_t>(), (int)B, (int)T, (int)V, accepted.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), ws.data_ptr(), (size_t)ws.numel(), d.stream()), "verify_drafts");
   }
   return {accepted, tokens};
 }

@@ -83,7 +83,8 @@ SIGNATURES = {
     "fgrpo_paged_cache_read": (_i, [_vp, _vp, _ll, _i, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     "fgrpo_paged_attn_workspace": (_sz, [_vp, _i, _i, _i, _i, _i]),
     "fgrpo_paged_attn_fwd": (_i, [_vp, _ll, _ll, _vp, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _sz, _vp]),
-    "fgrpo_verify_drafts": (_i, [_vp, _ll, _vp, _ll, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "fgrpo_verify_drafts_workspace": (_sz, [_i, _i]),
+    "fgrpo_verify_drafts": (_i, [_vp, _ll, _vp, _ll, _i, _i, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _sz, _vp]),
 }
 
 

@@ -441,10 +441,11 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
  * draft_n, 0) (where that is all zero, and behind K that stand, from target_n), then -1.  Drawn: the first x
  * whose running sum over the vocabulary exceeds u[cu[b]+n] times the sum, sums in 64 bits; values that are no probability
  * (negative, NaN, infinite) count as 0, and a row of zeros gives -1.  tokens behind cu[n_seq] are left as they are; a
- * sequence without rows has accepted 0.  No counterpart in the reference, whose engine samples by itself. */
+ * sequence without rows has accepted 0.  ws: 16-byte aligned, fgrpo_verify_drafts_workspace bytes, one per call in flight.  No counterpart in the reference, whose engine samples by itself. */
+size_t fgrpo_verify_drafts_workspace(int n_seq, int V);
 int fgrpo_verify_drafts(const void* target, long long target_stride, const void* draft, long long draft_stride, int draft_rows, int dtype,
                         const int64_t* ids, const float* u, const int32_t* cu_seqlens, int n_seq, int T, int V, int32_t* accepted,
-                        int64_t* tokens, void* stream);
+                        int64_t* tokens, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

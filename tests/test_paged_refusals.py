@@ -63,9 +63,9 @@ def test_attention_arguments(lib, over, rc):
 
 
 @pytest.mark.parametrize("at,value,rc", [(0, None, -1), (1, 10, -1), (3, 10, -1), (4, -1, -1), (5, 7, -1), (6, None, -1), (7, None, -1), (8, None, -1),
-                                         (9, 0, -1), (10, 0, -1), (11, 0, -1), (12, None, -1), (13, None, -1)])
+                                         (9, 0, -1), (10, 0, -1), (11, 0, -1), (11, 1 << 30, -1), (12, None, -1), (13, None, -1), (14, None, -3), (14, ODD, -5), (15, 8, -3)])
 def test_verify_arguments(lib, at, value, rc):
-    args = [AT, 1000, AT, 1000, 3, 1, AT, AT, AT, 2, 5, 1000, AT, AT, None]
+    args = [AT, 1000, AT, 1000, 3, 1, AT, AT, AT, 2, 5, 1000, AT, AT, AT, 1 << 40, None]
     args[at] = value
     assert lib.fgrpo_verify_drafts(*args) == rc and lib.fgrpo_last_error().startswith(b"verify_drafts: ")
 
