@@ -42,8 +42,8 @@ PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long ta
   v.k = (char*)c->k, v.v = (char*)c->v, v.k_scale = c->k_scale, v.v_scale = c->v_scale;
   for (int i = 0; i < 3; ++i)
     v.k_st[i] = c->k_stride[i], v.v_st[i] = c->v_stride[i], v.ks_st[i] = c->k_scale_stride[i], v.vs_st[i] = c->v_scale_stride[i];
-  v.table = table, v.lens = lens, v.cu = cu, v.table_st = table_st;
-  v.B = B, v.T = T, v.width = width, v.page_log2 = __builtin_ctz(c->block_size), v.num_pages = c->num_blocks, v.Hkv = c->heads;
+  v.table = width > 0 ? table : lens, v.lens = lens, v.cu = cu, v.table_st = width > 0 ? table_st : 0, v.reach = width * c->block_size;
+  v.B = B, v.T = T, v.width = width > 0 ? width : 1, v.page_log2 = __builtin_ctz(c->block_size), v.num_pages = c->num_blocks, v.Hkv = c->heads;
   return v;
 }
 
@@ -57,38 +57,47 @@ PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long ta
     HIP_TRY(hipGetLastError());                                                                                        \
   } while (0)
 
-// How a call is divided, from shapes alone.  rb: blocks of 32 rows a wavefront takes (0: work-groups of 128 rows).
-struct RowsPlan {
-  int rb, W;
+// How a call is divided, from shapes alone: rows of an item (16, 32, 64: one wavefront; 128: four) and work-groups.
+struct PagedPlan {
+  int rows, W, items;      // items: as in PagedSplit
+  int shape() const { return rows == 16 ? 16 : 32; }
+  size_t slots() const { return 2ull * W; }
+  size_t rec_bytes() const { return slots() * 2 * sizeof(int4); }
+  size_t part_bytes(int D) const { return slots() * rows * D * 4; }
+  size_t bytes(int D) const { return rec_bytes() + part_bytes(D) + slots() * rows * sizeof(float2); }
 };
-RowsPlan plan_rows(const fgrpo_paged_cache* c, int width, int n_seq, int T, int G, int max_len) {
-  const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq;      // not known: the mean
-  RowsPlan r{tokens * G <= 32 ? 1 : tokens * G <= 64 ? 2 : 0, 0};
-  const long long tiles = (long long)T * G / (r.rb ? 32 * r.rb : kPagedRows) + n_seq, steps = ((long long)width * c->block_size + 63) / 64 + 1;
-  long long W = (r.rb ? 4LL : 2LL) * num_cus();
-  if (tiles * c->heads < W && tiles * c->heads * steps < W) W = tiles * c->heads * steps;
+PagedPlan plan_paged(const fgrpo_paged_cache* c, int width, int n_seq, int T, int G, int max_len) {
+  const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq, rows = tokens * G;      // not known: the mean
+  PagedPlan r{rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedRows, 0, 0};
+  const long long items = ((long long)T * G / r.rows + n_seq) * c->heads, steps = ((long long)width * c->block_size + 63) / 64 + 1;
+  long long W = (r.rows <= 32 ? 4LL : 2LL) * num_cus();
+  if (items < W && items * steps < W) W = items * steps;
   r.W = (int)round_up(W, 8);
+  if (r.rows != kPagedRows && 8 * items <= r.W) r.items = (int)items;
   return r;
 }
-size_t rows_bytes(const RowsPlan& r, int D) { return 2ull * r.W * (sizeof(int4) + (r.rb ? r.rb : kPagedTileRB) * 32 * (D * 4 + sizeof(float2))); }
 
-template <int HD, bool FP8>
-int launch_attn(int rb, const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
-  if (rb == 1) {
-    hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 1>), dim3(sp.W), dim3(64), 0, st, p, sp);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((paged_merge_kernel<HD, FP8, 1, 1>), dim3(sp.W, HD / 32), dim3(256), 0, st, p, sp);
-  } else if (rb == 2) {
-    hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 2>), dim3(sp.W), dim3(64), 0, st, p, sp);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((paged_merge_kernel<HD, FP8, 2, 1>), dim3(sp.W, 2 * HD / 32), dim3(256), 0, st, p, sp);
-  } else {
-    hipLaunchKernelGGL((paged_tiles_kernel<HD, FP8>), dim3(sp.W), dim3(256), 0, st, p, sp);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL((paged_merge_kernel<HD, false, kPagedTileRB, HD / 32>), dim3(2 * sp.W, kPagedTileRB), dim3(256), 0, st, p, sp);
-  }
+template <int HD, bool PAIRS, int SHAPE, int RB>
+int launch_merge(const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
+  if (sp.items > 0)
+    hipLaunchKernelGGL((paged_merge_items_kernel<HD, PAIRS, SHAPE, RB>), dim3(sp.items, RB * HD / (SHAPE == 32 ? 8 : 16)), dim3(256), 0, st, p, sp);
+  else
+    hipLaunchKernelGGL((paged_merge_kernel<HD, PAIRS, SHAPE, RB>), dim3(sp.odd ? sp.W : 2 * sp.W, RB), dim3(256), 0, st, p, sp);
   HIP_TRY(hipGetLastError());
   return 0;
+}
+template <int HD, bool FP8>
+int launch_attn(const PagedPlan& plan, const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
+  const dim3 grid(sp.W);
+  if (plan.rows == 16) hipLaunchKernelGGL((paged_rows16_kernel<HD, FP8>), grid, dim3(64), 0, st, p, sp);
+  else if (plan.rows == 32) hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 1>), grid, dim3(64), 0, st, p, sp);
+  else if (plan.rows == 64) hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 2>), grid, dim3(64), 0, st, p, sp);
+  else hipLaunchKernelGGL((paged_tiles_kernel<HD, FP8>), grid, dim3(256), 0, st, p, sp);
+  HIP_TRY(hipGetLastError());
+  if (plan.rows == 16) return launch_merge<HD, FP8, 16, 1>(p, sp, st);
+  if (plan.rows == 32) return launch_merge<HD, FP8, 32, 1>(p, sp, st);
+  if (plan.rows == 64) return launch_merge<HD, FP8, 32, 2>(p, sp, st);
+  return launch_merge<HD, false, 32, kPagedTileRB>(p, sp, st);
 }
 
 int verify_chunks(int V) { return (V + kVerifyChunk - 1) / kVerifyChunk; }
@@ -141,7 +150,7 @@ int fgrpo_paged_cache_read(const fgrpo_paged_cache* cache, const int32_t* block_
 
 size_t fgrpo_paged_attn_workspace(const fgrpo_paged_cache* cache, int width, int n_seq, int T, int Hq, int max_len) {
   if (!cache || cache->heads <= 0 || Hq <= 0 || Hq % cache->heads || n_seq <= 0 || T <= 0 || width < 0 || (cache->head_dim != 128 && cache->head_dim != 64)) return 0;
-  return rows_bytes(plan_rows(cache, width, n_seq, T, Hq / cache->heads, max_len), cache->head_dim);
+  return plan_paged(cache, width, n_seq, T, Hq / cache->heads, max_len).bytes(cache->head_dim);
 }
 
 int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride_h, const fgrpo_paged_cache* cache, const int32_t* block_table,
@@ -162,22 +171,17 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
   p.c = view_of(cache, block_table, table_stride, width, seqused_k, cu_seqlens_q, n_seq, T);
   p.q = (const bf16_t*)q, p.q_t = q_stride_t, p.q_h = q_stride_h, p.out = (bf16_t*)out, p.lse = lse;
   p.scale = softmax_scale, p.Hq = Hq, p.G = G, p.causal = causal != 0;
-  const RowsPlan plan = plan_rows(cache, width, n_seq, T, G, max_len);
-  const size_t need = rows_bytes(plan, cache->head_dim);
+  const PagedPlan plan = plan_paged(cache, width, n_seq, T, G, max_len);
+  const size_t need = plan.bytes(cache->head_dim);
   if (!ws || ws_bytes < need) return fail(FGRPO_ERR_WORKSPACE, "paged_attn_fwd: workspace %zu < %zu", ws ? ws_bytes : 0, need);
   if (!aligned16(ws)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: workspace must be 16-byte aligned");
   PagedSplit sp;
-  const size_t slots = 2ull * plan.W;
-  sp.W = plan.W, sp.odd = plan.rb != 0;
+  sp.W = plan.W, sp.odd = plan.rows != kPagedRows, sp.items = plan.items, sp.most_parts = plan.items > 0 ? 1024 : 128;      // what a merge reads one behind the other
   sp.rec = (int4*)ws;
-  sp.part = (float*)((char*)ws + slots * sizeof(int4));
-  sp.ml = (float2*)((char*)sp.part + slots * (plan.rb ? plan.rb : kPagedTileRB) * 32 * cache->head_dim * 4);
-  if (cache->dtype == FGRPO_F8E4M3) {
-    if (cache->head_dim == 128) return launch_attn<128, true>(plan.rb, p, sp, st);
-    return launch_attn<64, true>(plan.rb, p, sp, st);
-  }
-  if (cache->head_dim == 128) return launch_attn<128, false>(plan.rb, p, sp, st);
-  return launch_attn<64, false>(plan.rb, p, sp, st);
+  sp.part = (float*)((char*)ws + plan.rec_bytes());
+  sp.ml = (float2*)((char*)sp.part + plan.part_bytes(cache->head_dim));
+  if (cache->dtype == FGRPO_F8E4M3) return cache->head_dim == 128 ? launch_attn<128, true>(plan, p, sp, st) : launch_attn<64, true>(plan, p, sp, st);
+  return cache->head_dim == 128 ? launch_attn<128, false>(plan, p, sp, st) : launch_attn<64, false>(plan, p, sp, st);
 }
 
 size_t fgrpo_verify_drafts_workspace(int n_seq, int V) {

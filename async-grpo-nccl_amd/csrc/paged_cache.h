@@ -23,17 +23,17 @@ struct PagedView {
   float* k_scale;        // null: bf16
   float* v_scale;
   long long k_st[3], v_st[3], ks_st[3], vs_st[3];      // page, token, head; elements
-  const int* table;      // [B][width], rows table_st apart
+  const int* table;      // [B][width], rows table_st apart (width >= 1: without a table, any readable address)
   const int* lens;       // [B]
   const int* cu;         // [B + 1]
   long long table_st;
-  int B, T, width, page_log2, num_pages, Hkv;
+  int B, T, width, reach, page_log2, num_pages, Hkv;      // reach: tokens that the table has blocks for
 };
 
 struct PagedSeq {
   int b, row0, rows, len;      // b < 0: the row belongs to no sequence
 };
-__device__ __forceinline__ int paged_len(const PagedView& c, int b) { return min(max(c.lens[b], 0), c.width << c.page_log2); }
+__device__ __forceinline__ int paged_len(const PagedView& c, int b) { return min(max(c.lens[b], 0), c.reach); }
 
 // The sequence of packed row t (the same in all lanes): 64 ends at a time.  cu is taken to ascend; rows from cu[B] on belong to none.
 __device__ __forceinline__ PagedSeq paged_find(const PagedView& c, int t, int lane) {

@@ -10,34 +10,35 @@
 
 namespace fgrpo {
 
-constexpr int kPagedMaxParts = 128;      // of an item: what the merge reads one behind the other
 
 struct PagedSplit {
   int W;                 // work-groups of the launch, a multiple of 8
-  int odd;               // only odd slots begin items
-  float* part;           // [2 W][row blocks][32 x HD] sums of a part, as attn_store_partial leaves them
-  float2* ml;            // [2 W][row blocks][32] maximum (in powers of two) and sum
-  int4* rec;             // [2 W] for the slot of an item's first part: {sequence + 1, tile, head, parts (negative: its slots are neighbours)}; 0: none
+  int odd;               // only odd slots begin items (shares alone)
+  int items;             // > 0: no more items than this, few enough for the merge to have work-groups for every unit of each: records go by item, not by slot
+  int most_parts;        // of an item
+  float* part;           // [2 W][row blocks][units][64 lanes][4] sums of a part (paged_column)
+  float2* ml;            // [2 W][rows] maximum (in powers of two) and sum
+  int4* rec;             // [2 W][2] for the slot of an item's first part, what its merge needs: {parts (0: none; negative: their slots are neighbours), first
+                         // packed row of the sequence, first row of the tile, rows of the sequence}, {head, its slot}
 };
 // slot of part i of an item whose first is in `slot`.  Shares: work-group w has 2 w for an item that an earlier one began and 2 w + 1 for one
 // that it begins and does not end.
 __device__ __forceinline__ int paged_slot(int slot, int i, bool neighbours) { return neighbours ? slot + i : i ? slot - 1 + 2 * i : slot; }
 
-// Weight of tile t (ROWS rows) of a sequence: whole numbers in doubles, exact below 2^53.
+// A sequence, and the weight of its tiles t (ROWS rows): whole numbers in doubles, exact below 2^53.
 struct PagedWeight {
+  int q0, nq, len;         // first packed row, rows, keys
+  int tiles;
   double base, slope;      // w_t = base + slope (t + 1)
-  int tiles, len, nq, q0;
   __device__ __forceinline__ double of(int t) const { return base + slope * (t + 1); }
   __device__ __forceinline__ double upto(int n) const { return base * n + slope * 0.5 * n * (n + 1.0); }      // tiles 0 .. n - 1
 };
 template <int ROWS>
-__device__ __forceinline__ PagedWeight paged_weight(const PagedAttn& p, int b) {
+__device__ __forceinline__ PagedWeight paged_weight(const PagedAttn& p, int q0, int nq, int len) {
   PagedWeight w;
-  w.q0 = min(max(p.c.cu[b], 0), p.c.T);
-  w.nq = min(max(p.c.cu[b + 1], w.q0), p.c.T) - w.q0;
-  w.len = paged_len(p.c, b);
-  w.tiles = (int)(((long long)w.nq * p.G + ROWS - 1) / ROWS);
-  w.base = (double)(p.causal ? max(w.len - w.nq, 0) : w.len) * p.G + ROWS;
+  w.q0 = q0, w.nq = nq, w.len = len;
+  w.tiles = (int)(((long long)nq * p.G + ROWS - 1) / ROWS);
+  w.base = (double)(p.causal ? max(len - nq, 0) : len) * p.G + ROWS;
   w.slope = p.causal ? ROWS : 0;
   return w;
 }
@@ -46,20 +47,61 @@ __device__ __forceinline__ double uniform(double x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)u), hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+// inclusive sums and maxima over the lanes up to this one (values of at least 0), as wave_sum_upto moves them
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <class F>
+__device__ __forceinline__ double wave_upto(double x, F f) {
+  x = f(x, moved<0x111, 0xf>(x)), x = f(x, moved<0x112, 0xf>(x)), x = f(x, moved<0x114, 0xf>(x)), x = f(x, moved<0x118, 0xf>(x));
+  x = f(x, moved<0x142, 0xa>(x)), x = f(x, moved<0x143, 0xc>(x));
+  return x;
+}
+__device__ __forceinline__ double wave_sums(double x) { return wave_upto(x, [](double a, double b) { return a + b; }); }
+__device__ __forceinline__ double wave_most(double x) { return wave_upto(x, [](double a, double b) { return fmax(a, b); }); }
+__device__ __forceinline__ double lane_of(double x, int l) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)u, l), hi = __builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), l);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// 64 sequences from b0 on, one a lane (behind the last: of no rows).  Read once; what a work-group needs of one of them comes out of the lane's registers.
+template <int ROWS>
+struct PagedLanes {
+  int b0, q0, nq, len;
+  __device__ __forceinline__ void load(const PagedAttn& p, int first) {
+    b0 = first;
+    const int b = first + (threadIdx.x & 63);
+    q0 = nq = len = 0;
+    if (b < p.c.B) {
+      q0 = min(max(p.c.cu[b], 0), p.c.T);
+      nq = min(max(p.c.cu[b + 1], q0), p.c.T) - q0;
+      len = paged_len(p.c, b);
+    }
+  }
+  __device__ __forceinline__ PagedWeight mine(const PagedAttn& p) const { return paged_weight<ROWS>(p, q0, nq, len); }
+  __device__ __forceinline__ PagedWeight of(const PagedAttn& p, int b) {      // b, the same in all lanes, is below B
+    if (b < b0 || b >= b0 + 64) load(p, b & ~63);
+    const int l = b - b0;
+    return paged_weight<ROWS>(p, __builtin_amdgcn_readlane(q0, l), __builtin_amdgcn_readlane(nq, l), __builtin_amdgcn_readlane(len, l));
+  }
+};
 struct PagedTotal {
   double weight, most, items;      // of all items; the heaviest; how many
 };
 template <int ROWS>
-__device__ __forceinline__ PagedTotal paged_total(const PagedAttn& p) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ PagedTotal paged_total(const PagedAttn& p, PagedLanes<ROWS>& lanes) {      // leaves the first 64 sequences
   PagedTotal s{0, 1, 0};
-  for (int b = lane; b < p.c.B; b += 64) {
-    const PagedWeight w = paged_weight<ROWS>(p, b);
-    if (w.tiles > 0) s.weight += w.upto(w.tiles) * p.c.Hkv, s.most = fmax(s.most, w.of(w.tiles - 1)), s.items += (double)w.tiles * p.c.Hkv;
+  for (int b0 = (p.c.B - 1) & ~63; b0 >= 0; b0 -= 64) {
+    lanes.load(p, b0);
+    const PagedWeight w = lanes.mine(p);
+    s.weight += lane_of(wave_sums(w.upto(w.tiles) * p.c.Hkv), 63);
+    s.items += lane_of(wave_sums((double)w.tiles * p.c.Hkv), 63);
+    s.most = fmax(s.most, lane_of(wave_most(w.tiles > 0 ? w.of(w.tiles - 1) : 0.0), 63));
   }
-#pragma unroll
-  for (int d = 32; d; d >>= 1)
-    s.weight += __shfl_xor(s.weight, d, 64), s.most = fmax(s.most, __shfl_xor(s.most, d, 64)), s.items += __shfl_xor(s.items, d, 64);
   return PagedTotal{uniform(s.weight), uniform(s.most), uniform(s.items)};
 }
 
@@ -69,35 +111,25 @@ struct PagedItem {
 };
 // The item that holds place `x` of the weights, or of the numbers.
 template <int ROWS, bool NUMBERS>
-__device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, double x) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, PagedLanes<ROWS>& lanes, double x) {
   PagedItem s{p.c.B, 0, 0, 0, 0};
   double weight = 0, number = 0;      // in front of the 64 at hand
   for (int b0 = 0; b0 < p.c.B; b0 += 64) {
-    const int b = b0 + lane;
-    double m = 0, n = 0;
-    if (b < p.c.B) {
-      const PagedWeight w = paged_weight<ROWS>(p, b);
-      m = w.upto(w.tiles) * p.c.Hkv, n = (double)w.tiles * p.c.Hkv;
-    }
-    double upto_m = m, upto_n = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double y = __shfl_up(upto_m, d, 64), z = __shfl_up(upto_n, d, 64);
-      if (lane >= d) upto_m += y, upto_n += z;
-    }
+    if (lanes.b0 != b0) lanes.load(p, b0);
+    const PagedWeight w = lanes.mine(p);
+    const double m = w.upto(w.tiles) * p.c.Hkv, n = (double)w.tiles * p.c.Hkv, upto_m = wave_sums(m), upto_n = wave_sums(n);
     const unsigned long long past = __ballot((NUMBERS ? number + upto_n : weight + upto_m) > x);      // the first lane past it holds the sequence
     if (past) {
-      const int l = __ffsll(past) - 1;
-      s.b = b0 + l;
-      s.at = weight + __shfl(upto_m - m, l, 64), s.index = number + __shfl(upto_n - n, l, 64);
+      const int at = __ffsll(past) - 1;
+      s.b = b0 + at;
+      s.at = weight + lane_of(upto_m - m, at), s.index = number + lane_of(upto_n - n, at);
       break;
     }
-    weight += __shfl(upto_m, 63, 64), number += __shfl(upto_n, 63, 64);
+    weight += lane_of(upto_m, 63), number += lane_of(upto_n, 63);
   }
   s.b = __builtin_amdgcn_readfirstlane(s.b);
   if (s.b >= p.c.B) return PagedItem{p.c.B, 0, 0, uniform(weight), uniform(number)};
-  const PagedWeight w = paged_weight<ROWS>(p, s.b);
+  const PagedWeight w = lanes.of(p, s.b);
   const double one = NUMBERS ? (double)w.tiles : w.upto(w.tiles);      // of one head
   double r = x - (NUMBERS ? s.index : s.at);
   int head = (int)fmin(floor(r / one), p.c.Hkv - 1.0), t = 0;
@@ -118,14 +150,14 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, double x) {
   return s;
 }
 template <int ROWS>
-__device__ __forceinline__ void paged_next(const PagedAttn& p, PagedItem& s, const PagedWeight& w) {
-  s.at = uniform(s.at + w.of(s.t));
+__device__ __forceinline__ void paged_next(const PagedAttn& p, PagedLanes<ROWS>& lanes, PagedItem& s) {
+  const PagedWeight w = lanes.of(p, s.b);
+  s.at = uniform(s.at + w.of(s.t)), s.index = uniform(s.index + 1);
   if (++s.t < w.tiles) return;
   s.t = 0;
   if (++s.head < p.c.Hkv) return;
   s.head = 0;
-  do ++s.b; while (s.b < p.c.B && paged_weight<ROWS>(p, s.b).tiles == 0);
-  s.b = __builtin_amdgcn_readfirstlane(s.b);
+  do ++s.b; while (s.b < p.c.B && lanes.of(p, s.b).tiles == 0);
 }
 
 // Shares: work-group `at` of `used` has the weights [bound(at), bound(at + 1)).
@@ -139,8 +171,8 @@ struct PagedShares {
     return __builtin_amdgcn_readfirstlane(w);
   }
 };
-__device__ __forceinline__ PagedShares paged_shares(const PagedTotal& t, int W, double least) {      // least: weight that is worth a work-group
-  const double used = fmin(fmin((double)W, ceil(t.weight / least)), floor(t.weight * (kPagedMaxParts - 2) / t.most));
+__device__ __forceinline__ PagedShares paged_shares(const PagedTotal& t, int W, int most_parts, double least) {      // least: weight that is worth a work-group
+  const double used = fmin(fmin((double)W, ceil(t.weight / least)), floor(t.weight * (most_parts - 2) / t.most));
   return PagedShares{t.weight, uniform(fmax(used, 1.0))};
 }
 // what a work-group walks of an item, in steps of KB keys: places x0 .. x1 of its weight
@@ -168,9 +200,18 @@ __device__ __forceinline__ int paged_table_at(const PagedView& c, int b, int i) 
 }
 __device__ __forceinline__ float paged_lse(float m, float l) { return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY; }
 
-// Columns that a lane's accumulator values are.  Value r of block db: column 32 db + 8 (r / 4) + 4 h + r % 4.  PAIRS (the transposing reads moved
-// pairs of e4m3 codes): blocks 2 n and 2 n + 1 hold the even and the odd columns of 64, value r is column
-// 64 n + 2 (8 (r / 4) + 4 h + r % 4) + (block % 2), and the values of both blocks with r / 4 = g are eight neighbours.
+// What a lane's accumulators hold.  SHAPE: rows of a block, 32 (v_mfma_f32_32x32x16_bf16) or 16 (16x16x32); the lane has row lane % SHAPE and, in unit u, four
+// columns: in blocks of 32 columns value 4 g + i of block db is unit 4 db + g, in blocks of 16 value i of block u is unit u.  PAIRS (the transposing reads
+// moved pairs of e4m3 codes): blocks 2 n and 2 n + 1 hold the even and the odd columns of a range.
+template <int SHAPE, bool PAIRS>
+__device__ __forceinline__ int paged_column(int u, int lane) {      // of the unit's first value; the others are 1 (PAIRS: 2) apart
+  if constexpr (SHAPE == 32) {
+    const int db = u / 4, g = u % 4, h = lane >> 5;
+    return PAIRS ? 64 * (db / 2) + 16 * g + 8 * h + db % 2 : 8 * u + 4 * h;
+  } else {
+    return PAIRS ? 32 * (u / 2) + 8 * (lane >> 4) + u % 2 : 16 * u + 4 * (lane >> 4);
+  }
+}
 template <int HD, bool PAIRS>
 __device__ __forceinline__ void paged_store_row(const f32x16_t (&acc)[HD / 32], float mul, bf16_t* row, int h) {
   if constexpr (!PAIRS) {
@@ -188,63 +229,99 @@ __device__ __forceinline__ void paged_store_row(const f32x16_t (&acc)[HD / 32], 
   }
 }
 
-// Adds up the parts of the item whose first is in slot blockIdx.x, in the order of the keys: work-group y takes 32 rows and NC / DB of their
-// columns, a thread four columns of a row at a time.  RB: blocks of 32 rows of a tile.
-template <int HD, bool PAIRS, int RB, int NC>
-static __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p, PagedSplit sp) {
-  constexpr int DB = HD / 32, ROWS = 32 * RB, WIDE = 4;
-  const int first = sp.odd ? 2 * blockIdx.x + 1 : blockIdx.x, lane = threadIdx.x & 63, h = lane >> 5, g = threadIdx.x >> 6;
-  const int4 head = sp.rec[first];
-  if (head.x == 0) return;
-  const bool neighbours = head.w < 0;
-  const int np = neighbours ? -head.w : head.w;
-  const int b = min(max(head.x - 1, 0), p.c.B - 1), rb = blockIdx.y / (DB / NC), db0 = blockIdx.y % (DB / NC) * NC;
-  const int q0 = min(max(p.c.cu[b], 0), p.c.T), nq = min(max(p.c.cu[b + 1], q0), p.c.T) - q0;
-  const int row = head.y * ROWS + 32 * rb + (lane & 31);
-  if (row >= nq * p.G) return;
-  const int tok = q0 + row / p.G, hq = head.z * p.G + row % p.G;
-  float m = -INFINITY, l = 0.f;
-  float4 o[NC];
+struct PagedSum {
+  float m, l;              // maximum (in powers of two) and sum
+  float4 o;
+};
+__device__ __forceinline__ PagedSum paged_add(const PagedSum& a, const PagedSum& b) {
+  const float m = fmaxf(a.m, b.m), m_use = m == -INFINITY ? 0.f : m, x = fast_exp2(a.m - m_use), y = fast_exp2(b.m - m_use);
+  return PagedSum{m, a.l * x + b.l * y, make_float4(a.o.x * x + b.o.x * y, a.o.y * x + b.o.y * y, a.o.z * x + b.o.z * y, a.o.w * x + b.o.w * y)};
+}
+template <int SHAPE, bool PAIRS>
+__device__ __forceinline__ void paged_store_unit(bf16_t* row, int unit, int lane, const float4& o, float inv) {
+  bf16_t* dst = row + paged_column<SHAPE, PAIRS>(unit, lane);
+  if constexpr (PAIRS) {
+    dst[0] = f32_to_bf16_rn(o.x * inv), dst[2] = f32_to_bf16_rn(o.y * inv), dst[4] = f32_to_bf16_rn(o.z * inv), dst[6] = f32_to_bf16_rn(o.w * inv);
+  } else {
+    uint2 x;
+    x.x = pack_bf16x2(o.x * inv, o.y * inv), x.y = pack_bf16x2(o.z * inv, o.w * inv);
+    *(uint2*)dst = x;
+  }
+}
+
+// The same for few items of perhaps many parts: work-group (item, unit of a block of rows), its wavefronts taking parts w, w + 4 ..
+template <int HD, bool PAIRS, int SHAPE, int RB>
+static __global__ __launch_bounds__(256) void paged_merge_items_kernel(PagedAttn p, PagedSplit sp) {
+  constexpr int UNITS = HD / (SHAPE == 32 ? 8 : 16), WIDE = 8;
+  __shared__ PagedSum sh[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rb = blockIdx.y / UNITS, unit = blockIdx.y % UNITS;
+  const int4 rec = sp.rec[2 * blockIdx.x], place = sp.rec[2 * blockIdx.x + 1];
+  if (rec.x == 0) return;
+  const bool neighbours = rec.x < 0;
+  const int np = neighbours ? -rec.x : rec.x, row = rec.z + SHAPE * rb + lane % SHAPE;
+  const float* part = sp.part + (long long)rb * (SHAPE * HD) + (64 * unit + lane) * 4;
+  const float2* ml = sp.ml + rb * SHAPE + lane % SHAPE;
+  PagedSum sum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  if (row < rec.w)
+    for (int i0 = wave; i0 < np; i0 += 4 * WIDE) {
+      PagedSum x[WIDE];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  const float* part = sp.part + (long long)rb * (32 * HD) + (64 * (4 * db0 + g) + lane) * 4;
-  const float2* ml = sp.ml + rb * 32 + (lane & 31);
+      for (int i = 0; i < WIDE; ++i) {
+        const long long slot = (long long)RB * min(paged_slot(place.y, min(i0 + 4 * i, np - 1), neighbours), 2 * sp.W - 1);
+        const float2 y = ml[slot * SHAPE];
+        x[i] = PagedSum{y.x, y.y, *(const float4*)(part + slot * (SHAPE * HD))};
+      }
+#pragma unroll
+      for (int i = 0; i < WIDE; ++i)
+        if (i0 + 4 * i < np) sum = paged_add(sum, x[i]);
+    }
+  sh[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0 || row >= rec.w) return;
+  for (int i = 1; i < 4; ++i) sum = paged_add(sum, sh[i][lane]);
+  const int tok = rec.y + row / p.G, hq = place.x * p.G + row % p.G;
+  paged_store_unit<SHAPE, PAIRS>(p.out + ((long long)tok * p.Hq + hq) * HD, unit, lane, sum.o, sum.l > 0.f ? 1.f / sum.l : 0.f);
+  if (p.lse && unit == 0 && lane < SHAPE) p.lse[(long long)hq * p.c.T + tok] = paged_lse(sum.m, sum.l);
+}
+
+// Adds up the parts of the item whose first is in slot blockIdx.x (2 blockIdx.x + 1: only odd ones begin items), in the order of the keys: work-group y takes
+// block y of SHAPE rows, wavefront w the units w, w + 4 .. of their columns.  RB: blocks of a tile.
+template <int HD, bool PAIRS, int SHAPE, int RB>
+static __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p, PagedSplit sp) {
+  constexpr int NU = HD / (SHAPE == 32 ? 8 : 16) / 4, WIDE = 16 / NU < 8 ? 16 / NU : 8;
+  const int first = sp.odd ? 2 * blockIdx.x + 1 : blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rb = blockIdx.y;
+  const int4 rec = sp.rec[2 * first];
+  const int head = sp.rec[2 * first + 1].x;
+  if (rec.x == 0) return;
+  const bool neighbours = rec.x < 0;
+  const int np = neighbours ? -rec.x : rec.x, row = rec.z + SHAPE * rb + lane % SHAPE;
+  if (row >= rec.w) return;
+  const int tok = rec.y + row / p.G, hq = head * p.G + row % p.G;
+  PagedSum sum[NU];
+#pragma unroll
+  for (int c = 0; c < NU; ++c) sum[c] = PagedSum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  const float* part = sp.part + (long long)rb * (SHAPE * HD) + (64 * wave + lane) * 4;
+  const float2* ml = sp.ml + rb * SHAPE + lane % SHAPE;
   for (int i0 = 0; i0 < np; i0 += WIDE) {
     float2 x[WIDE];
-    float4 y[WIDE][NC];
+    float4 y[WIDE][NU];
 #pragma unroll
     for (int i = 0; i < WIDE; ++i) {
       const long long slot = (long long)RB * min(paged_slot(first, min(i0 + i, np - 1), neighbours), 2 * sp.W - 1);
-      x[i] = ml[slot * 32];
+      x[i] = ml[slot * SHAPE];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) y[i][c] = *(const float4*)(part + slot * (32 * HD) + 1024 * c);
+      for (int c = 0; c < NU; ++c) y[i][c] = *(const float4*)(part + slot * (SHAPE * HD) + 1024 * c);
     }
 #pragma unroll
-    for (int i = 0; i < WIDE; ++i) {
-      if (i0 + i >= np) break;
-      const float m_new = fmaxf(m, x[i].x), m_use = m_new == -INFINITY ? 0.f : m_new, a = fast_exp2(m - m_use), e = fast_exp2(x[i].x - m_use);
-      l = l * a + x[i].y * e;
+    for (int i = 0; i < WIDE; ++i)
+      if (i0 + i < np)
 #pragma unroll
-      for (int c = 0; c < NC; ++c)
-        o[c] = make_float4(o[c].x * a + y[i][c].x * e, o[c].y * a + y[i][c].y * e, o[c].z * a + y[i][c].z * e, o[c].w * a + y[i][c].w * e);
-      m = m_new;
-    }
+        for (int c = 0; c < NU; ++c) sum[c] = paged_add(sum[c], PagedSum{x[i].x, x[i].y, y[i][c]});
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  bf16_t* dst = p.out + ((long long)tok * p.Hq + hq) * HD;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int db = db0 + c;
-    if constexpr (PAIRS) {
-      const int col = 64 * (db / 2) + 2 * (8 * g + 4 * h) + db % 2;
-      dst[col] = f32_to_bf16_rn(o[c].x * inv), dst[col + 2] = f32_to_bf16_rn(o[c].y * inv), dst[col + 4] = f32_to_bf16_rn(o[c].z * inv), dst[col + 6] = f32_to_bf16_rn(o[c].w * inv);
-    } else {
-      uint2 x;
-      x.x = pack_bf16x2(o[c].x * inv, o[c].y * inv), x.y = pack_bf16x2(o[c].z * inv, o[c].w * inv);
-      *(uint2*)(dst + 32 * db + 8 * g + 4 * h) = x;
-    }
-  }
-  if (p.lse && db0 == 0 && g == 0 && h == 0) p.lse[(long long)hq * p.c.T + tok] = paged_lse(m, l);
+  for (int c = 0; c < NU; ++c)
+    paged_store_unit<SHAPE, PAIRS>(p.out + ((long long)tok * p.Hq + hq) * HD, wave + 4 * c, lane, sum[c].o, sum[c].l > 0.f ? 1.f / sum[c].l : 0.f);
+  if (p.lse && threadIdx.x < SHAPE) p.lse[(long long)hq * p.c.T + tok] = paged_lse(sum[0].m, sum[0].l);
 }
 
 }  // namespace fgrpo

@@ -41,7 +41,8 @@ template <int HD, bool FP8>
 static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p, PagedSplit sp) {
   using C = PagedTiles<HD, FP8>;
   constexpr int KS = HD / 16, DB = HD / 32, G4 = KS / 2, ROWS = kPagedRows;
-  __shared__ __attribute__((aligned(16))) char smem[C::LDS];
+  __shared__ __attribute__((aligned(1024))) char smem[C::LDS];      // fragment addresses are formed by flipping bits below 1024
+  __shared__ double kept[3];
   const uint32_t lds0 = lds_addr(smem);
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int xcd = blockIdx.x & 7, n = sp.W >> 3, me = blockIdx.x >> 3, w = xcd * n + me;
@@ -67,7 +68,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
   auto walk = [&](const PagedItem& s, const PagedWeight& wt, double x0, double x1, int slot) {
     const double weight = wt.of(s.t);
     const bool whole = x0 <= 0 && x1 >= weight;
-    const int q0 = __builtin_amdgcn_readfirstlane(wt.q0), nq = __builtin_amdgcn_readfirstlane(wt.nq), len = __builtin_amdgcn_readfirstlane(wt.len);
+    const int q0 = wt.q0, nq = wt.nq, len = wt.len;
     const int rows = nq * p.G, r0 = s.t * ROWS, rw = r0 + 32 * wave;
     const int k_end = __builtin_amdgcn_readfirstlane(paged_sight(p, wt, r0, ROWS).most);
     const PagedRange kr = paged_range<kAttnBK>(x0, x1, weight, k_end);
@@ -290,71 +291,76 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     const float l = l_lo + l_hi;
     int lane_e = lane;
     asm volatile("" : "+v"(lane_e));      // the row's addresses formed anew: held across the loop, they would cost registers
-    const int row_e = rw + (lane_e & 31), tok_e = q0 + row_e / p.G, hq_e = s.head * p.G + row_e % p.G;
+    const int h_e = lane_e >> 5, row_e = rw + (lane_e & 31), tok_e = q0 + row_e / p.G, hq_e = s.head * p.G + row_e % p.G;
     if (row_e >= rows) return;
     if (whole) {
-      attn_store_rowmajor(acc, l > 0.f ? 1.f / l : 0.f, p.out + ((long long)tok_e * p.Hq + hq_e) * HD, h);
-      if (p.lse && h == 0) p.lse[(long long)hq_e * p.c.T + tok_e] = paged_lse(m_run, l);
+      attn_store_rowmajor(acc, l > 0.f ? 1.f / l : 0.f, p.out + ((long long)tok_e * p.Hq + hq_e) * HD, h_e);
+      if (p.lse && h_e == 0) p.lse[(long long)hq_e * p.c.T + tok_e] = paged_lse(m_run, l);
     } else {
       attn_store_partial(acc, sp.part + ((long long)slot * kPagedTileRB + wave) * (32 * HD), lane_e);
-      if (h == 0) sp.ml[((long long)slot * kPagedTileRB + wave) * 32 + lane_e] = make_float2(m_run, l);
+      if (h_e == 0) sp.ml[((long long)slot * kPagedTileRB + wave) * 32 + lane_e] = make_float2(m_run, l);
     }
   };
 
-  const PagedTotal total = paged_total<ROWS>(p);
+  PagedLanes<ROWS> lanes;
+  const PagedTotal total = paged_total<ROWS>(p, lanes);
   const int4 none = make_int4(0, 0, 0, 0);
   const bool shares = total.items < sp.W || total.most * sp.W > 2 * total.weight;
-  const PagedShares sh = paged_shares(total, sp.W, 2.0 * kAttnBK * p.G);
+  PagedShares sh = paged_shares(total, sp.W, sp.most_parts, 2.0 * kAttnBK * p.G);
   double done = 0, hi = 0;                                    // shares: this one
   int first = 0, rounds = 0, left = 0, parts = 1, turn = 0;      // whole items: the XCD's first, rounds of n, those of the last round, their parts; this work-group's turn
   PagedItem s{0, 0, 0, 0, 0};
   if (shares) {
-    if (threadIdx.x == 0) sp.rec[2 * w] = sp.rec[2 * w + 1] = none;
+    if (threadIdx.x == 0) sp.rec[4 * w] = sp.rec[4 * w + 2] = none;
     if (!(w < sh.used)) return;
     done = sh.bound(w), hi = sh.bound(w + 1);
     if (!(done < hi)) return;
-    s = paged_item<ROWS, false>(p, done);
+    s = paged_item<ROWS, false>(p, lanes, done);
   } else {                       // those that begin in this XCD's eighth of the weights
-    if (threadIdx.x == 0) sp.rec[2 * n * xcd + me] = sp.rec[2 * n * xcd + n + me] = none;
-    first = __builtin_amdgcn_readfirstlane((int)paged_item<ROWS, false>(p, floor(total.weight * xcd / 8)).index);
-    const int last = xcd == 7 ? (int)total.items : (int)paged_item<ROWS, false>(p, floor(total.weight * (xcd + 1) / 8)).index;
+    if (threadIdx.x == 0) sp.rec[2 * (2 * n * xcd + me)] = sp.rec[2 * (2 * n * xcd + n + me)] = none;
+    first = __builtin_amdgcn_readfirstlane((int)paged_item<ROWS, false>(p, lanes, floor(total.weight * xcd / 8)).index);
+    const int last = xcd == 7 ? (int)total.items : (int)paged_item<ROWS, false>(p, lanes, floor(total.weight * (xcd + 1) / 8)).index;
     const int items = __builtin_amdgcn_readfirstlane(last) - first;
     rounds = items / n, left = items - rounds * n, parts = __builtin_amdgcn_readfirstlane(paged_last_parts(left, n));
   }
+  if (threadIdx.x == 0) kept[0] = sh.total, kept[1] = sh.used, kept[2] = hi;      // what the walks must not carry in registers
+  __syncthreads();
   for (;;) {
     double x0 = 0, x1;
     int slot = 0, part = 0;
     if (!shares) {
       if (turn < rounds) {
-        s = paged_item<ROWS, true>(p, first + turn * n + (turn & 1 ? n - 1 - me : me));
+        s = paged_item<ROWS, true>(p, lanes, first + turn * n + (turn & 1 ? n - 1 - me : me));
       } else {
         const int i = (turn - rounds) * n + me;
         if (i >= left * parts || turn - rounds > 1) break;
-        s = paged_item<ROWS, true>(p, first + rounds * n + i / parts);
+        s = paged_item<ROWS, true>(p, lanes, first + rounds * n + i / parts);
         slot = 2 * n * xcd + i, part = i % parts;
       }
       ++turn;
     }
     if (s.b >= p.c.B) break;
-    const PagedWeight wt = paged_weight<ROWS>(p, s.b);
+    const PagedWeight wt = lanes.of(p, s.b);
     const double weight = wt.of(s.t);
-    int4 rec = none;
+    int rec = 0;               // parts, where this is an item's first of several
     if (shares) {
       x0 = done - s.at, x1 = fmin(hi - s.at, weight);
       slot = 2 * w + (x0 <= 0);
-      if (x0 <= 0 && x1 < weight) rec = make_int4(s.b + 1, s.t, s.head, sh.holding(s.at + weight - 1) - w + 1);
+      if (x0 <= 0 && x1 < weight) rec = sh.holding(s.at + weight - 1) - w + 1;
     } else if (turn > rounds) {
       x0 = floor(weight * part / parts), x1 = floor(weight * (part + 1) / parts);
-      if (parts > 1 && part == 0) rec = make_int4(s.b + 1, s.t, s.head, -parts);
+      if (parts > 1 && part == 0) rec = -parts;
     } else {
       x1 = weight;
     }
-    if (rec.x != 0 && threadIdx.x == 0) sp.rec[slot] = rec;
+    if (rec != 0 && threadIdx.x == 0) sp.rec[2 * slot] = make_int4(rec, wt.q0, s.t * ROWS, wt.nq * p.G), sp.rec[2 * slot + 1] = make_int4(s.head, slot, 0, 0);
     walk(s, wt, x0, x1, slot);
+    lanes.b0 = -64;            // read again, as these are
+    sh.total = uniform(kept[0]), sh.used = uniform(kept[1]), hi = uniform(kept[2]);
     if (shares) {
-      paged_next<ROWS>(p, s, paged_weight<ROWS>(p, s.b));
-      done = s.at;
+      done = uniform(s.at + weight);
       if (!(done < hi)) break;
+      paged_next<ROWS>(p, lanes, s);
     }
   }
 }

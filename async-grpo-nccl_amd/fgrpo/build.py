@@ -29,7 +29,10 @@ SOURCES = ["fgrpo_api.hip", "launch_lmhead.hip", "launch_gemm.hip", "launch_attn
 # instructions it schedules itself into a[0:15], over the first accumulator, spilling nothing.  The define lets the
 # source refuse a compilation without the flag; whether the compiler kept out is read off its assembly
 # (check_named_accumulators).
-SOURCE_FLAGS = {"launch_attn_keyside.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-DFGRPO_MFMA_VGPR_FORM=1"]}
+SOURCE_FLAGS = {"launch_attn_keyside.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-DFGRPO_MFMA_VGPR_FORM=1"],
+                # no named registers here: kernels of one wavefront per SIMD would have their accumulators in accumulation registers, and
+                # move them for each rescale and each soft-max
+                "launch_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 NAMED_ACCUMULATORS = {"launch_attn_keyside.hip": "varlen_attn_dkv3_kernel"}
 
 HIPCC_FLAGS = [
