@@ -57,7 +57,7 @@ PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long ta
     HIP_TRY(hipGetLastError());                                                                                        \
   } while (0)
 
-// How a call is divided, from shapes alone: rows of an item (16, 32, 64: one wavefront; 128: four) and work-groups.
+// How a call is divided, from shapes alone: rows of an item (16, 32: one wavefront; 128: four) and work-groups.
 struct PagedPlan {
   int rows, W, items;      // items: as in PagedSplit
   int shape() const { return rows == 16 ? 16 : 32; }
@@ -68,9 +68,9 @@ struct PagedPlan {
 };
 PagedPlan plan_paged(const fgrpo_paged_cache* c, int width, int n_seq, int T, int G, int max_len) {
   const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq, rows = tokens * G;      // not known: the mean
-  PagedPlan r{rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : kPagedRows, 0, 0};
+  PagedPlan r{rows <= 16 ? 16 : rows <= 64 ? 32 : kPagedRows, 0, 0};
   const long long items = ((long long)T * G / r.rows + n_seq) * c->heads, steps = ((long long)width * c->block_size + 63) / 64 + 1;
-  long long W = (r.rows <= 32 ? 4LL : 2LL) * num_cus();
+  long long W = (r.rows == kPagedRows ? 2LL : 4LL) * num_cus();
   if (items < W && items * steps < W) W = items * steps;
   r.W = (int)round_up(W, 8);
   if (r.rows != kPagedRows && 8 * items <= r.W) r.items = (int)items;
@@ -90,13 +90,11 @@ template <int HD, bool FP8>
 int launch_attn(const PagedPlan& plan, const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
   const dim3 grid(sp.W);
   if (plan.rows == 16) hipLaunchKernelGGL((paged_rows16_kernel<HD, FP8>), grid, dim3(64), 0, st, p, sp);
-  else if (plan.rows == 32) hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 1>), grid, dim3(64), 0, st, p, sp);
-  else if (plan.rows == 64) hipLaunchKernelGGL((paged_rows_kernel<HD, FP8, 2>), grid, dim3(64), 0, st, p, sp);
+  else if (plan.rows == 32) hipLaunchKernelGGL((paged_rows_kernel<HD, FP8>), grid, dim3(64), 0, st, p, sp);
   else hipLaunchKernelGGL((paged_tiles_kernel<HD, FP8>), grid, dim3(256), 0, st, p, sp);
   HIP_TRY(hipGetLastError());
   if (plan.rows == 16) return launch_merge<HD, FP8, 16, 1>(p, sp, st);
   if (plan.rows == 32) return launch_merge<HD, FP8, 32, 1>(p, sp, st);
-  if (plan.rows == 64) return launch_merge<HD, FP8, 32, 2>(p, sp, st);
   return launch_merge<HD, false, 32, kPagedTileRB>(p, sp, st);
 }
 

@@ -2,7 +2,7 @@
 // j < k_b, and with the causal mask j <= k_b - q_b + i.  o = softmax(c q K^T) V over what it sees; nothing seen: o = 0, lse = -inf.
 //
 // The G query heads of a K/V head read the same keys, so rows are (token, head of the group) pairs, row r of a sequence being token
-// r / G, head r mod G: tiles of rows are full whatever G is.  A wavefront has 32 rows (paged_tiles.h) or 32 and 64 (paged_rows.h) and
+// r / G, head r mod G: tiles of rows are full whatever G is.  A wavefront has 32 rows (paged_tiles.h) or 16 and 32 (paged_rows.h) and
 // computes S^T = K Q^T and O^T = V^T P^T with the matrix instruction's operands as the packed attention has them (attn_kernels.h): a lane owns one
 // row, and its probabilities are the next product's operand as they lie.
 // An e4m3 cache: codes are exact in bf16, so the products take them as they are; a key's scale multiplies its scores (exactly as

@@ -1,7 +1,7 @@
 // Attention over a paged cache for few rows a sequence (single tokens, drafts): all of its time is reading the cache, so the work is
 // dealt out by what is read.  (What is computed: paged_attn.h.)
 //
-// A work-group is one wavefront.  It owns ROWS = 16, 32 or 64 rows of a sequence and K/V head (G rows a token) and a stretch of the
+// A work-group is one wavefront.  It owns ROWS = 16 or 32 rows of a sequence and K/V head (G rows a token) and a stretch of the
 // keys, which it walks in steps of KB = 32 or 64: a step's K and V travel global -> LDS directly, a step ahead.  No barriers.  The pages of a step are looked up by the scalar unit, a step
 // ahead of their loads: 16 tokens that start at a multiple of 16 lie in one page, so each such group is one buffer descriptor, whose
 // length ends with the stretch - rows behind it arrive as zeros, whatever lies there.
@@ -159,7 +159,7 @@ __device__ __forceinline__ float paged_sum_of_four(float x) {
 }
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------
-template <int HD, bool FP8, int ROWS>
+template <int HD, bool FP8>
 struct PagedRows {
   static constexpr int ES = FP8 ? 1 : 2, RBY = HD * ES, NB = RBY == 256 ? 1 : 2, KB = 32 * NB, NG = KB / 16;
   static constexpr int CPR = RBY / 16, RPI = 1024 / RBY, IPG = 16 / RPI;
@@ -287,7 +287,7 @@ struct PagedWalk {
 // Blocks of 16 rows: a token of up to 16 query heads a K/V head.  Half the arithmetic of a block of 32, and half the registers.
 template <int HD, bool FP8>
 static __global__ __launch_bounds__(64) void paged_rows16_kernel(PagedAttn p, PagedSplit sp) {
-  using C = PagedRows<HD, FP8, 16>;
+  using C = PagedRows<HD, FP8>;
   constexpr int KS = HD / 32, DB = HD / 16, NK = C::RBY / 64, NV = C::RBY / 32;      // instructions of a score; blocks of columns; chunks and column blocks of a row as it lies
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];      // fragment addresses are formed by flipping bits below 1024
   const uint32_t lds0 = lds_addr(smem);
@@ -429,49 +429,40 @@ static __global__ __launch_bounds__(64) void paged_rows16_kernel(PagedAttn p, Pa
   });
 }
 
-// Blocks of 32 rows, RB of them.
-template <int HD, bool FP8, int RB>
+// Blocks of 32 rows: drafts.  Up to 64 rows a K/V head take two of them, which read the same keys out of one L2.  (64 rows a wavefront, K and V
+// read once, need all registers of a SIMD and have their arithmetic in one wavefront: 1 to 8 drafts of 14 / 2 heads of 64 30 us
+// against 25, of 40 / 8 heads of 128 54 against 52, in e4m3 63 against 43.)
+template <int HD, bool FP8>
 static __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttn p, PagedSplit sp) {
-  constexpr int ROWS = 32 * RB;
-  using C = PagedRows<HD, FP8, ROWS>;
+  using C = PagedRows<HD, FP8>;
   constexpr int KS = HD / 16, DB = HD / 32, VB = C::RBY / 64;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];      // fragment addresses are formed by flipping bits below 1024
   const uint32_t lds0 = lds_addr(smem);
-  PagedWalk<C, ROWS> W(p, sp, [](int row) { return paged_swz<C::RBY>(row); });
+  PagedWalk<C, 32> W(p, sp, [](int row) { return paged_swz<C::RBY>(row); });
   const int lane = W.lane, h = lane >> 5;
   const PagedLane<C::RBY> L = paged_lane<C::RBY>(lane, lds0);
   const float c = p.scale * kLog2e;
   W.run([&]() {
-    int seen[RB];
-    bf16x8_t qf[RB][KS];         // chunks as the K fragments have theirs (e4m3: 16 bytes are two steps' worth)
+    const int row = min(W.r0 + (lane & 31), W.rows - 1), tok = row / p.G, hq = W.head * p.G + row % p.G;      // lanes behind the last row repeat it
+    const int seen = p.causal ? min(max(W.len - W.nq + tok + 1, 0), W.len) : W.len;
+    bf16x8_t qf[KS];             // chunks as the K fragments have theirs (e4m3: 16 bytes are two steps' worth)
+    const bf16_t* src = p.q + (long long)(W.q0 + tok) * p.q_t + (long long)hq * p.q_h;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const int row = min(W.r0 + 32 * rb + (lane & 31), W.rows - 1), tok = row / p.G;      // lanes behind the last row repeat it
-      seen[rb] = p.causal ? min(max(W.len - W.nq + tok + 1, 0), W.len) : W.len;
-      const bf16_t* src = p.q + (long long)(W.q0 + tok) * p.q_t + (long long)(W.head * p.G + row % p.G) * p.q_h;
-#pragma unroll
-      for (int st = 0; st < KS; ++st) qf[rb][st] = *(const bf16x8_t*)(src + (FP8 ? 4 * (st / 2) + 2 * h + st % 2 : 2 * st + h) * 8);
-    }
+    for (int st = 0; st < KS; ++st) qf[st] = *(const bf16x8_t*)(src + (FP8 ? 4 * (st / 2) + 2 * h + st % 2 : 2 * st + h) * 8);
     __builtin_amdgcn_sched_barrier(0);
     W.prologue(smem);
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {      // as in the kernel for 16
-        u32x4_t x = __builtin_bit_cast(u32x4_t, qf[rb][st]);
-        attn_settle(x);
-        qf[rb][st] = __builtin_bit_cast(bf16x8_t, x);
-      }
-    f32x16_t acc[RB][DB];
-    float m_run[RB], l_run[RB];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      m_run[rb] = -INFINITY, l_run[rb] = 0.f;
-#pragma unroll
-      for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[rb][db][r] = 0.f;
+    for (int st = 0; st < KS; ++st) {      // as in the kernel for 16
+      u32x4_t x = __builtin_bit_cast(u32x4_t, qf[st]);
+      attn_settle(x);
+      qf[st] = __builtin_bit_cast(bf16x8_t, x);
     }
+    f32x16_t acc[DB];
+    float m_run = -INFINITY, l_run = 0.f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
     __builtin_amdgcn_sched_barrier(0);
     auto step = [&](auto curc, int kb) {
       constexpr int cur = decltype(curc)::value, base = cur * C::BUF;
@@ -485,65 +476,54 @@ static __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttn p, Page
           paged_read_scales<cur * 2 * C::KB * 4 + mb * 128>(sk, lds0 + C::SCALES + 16 * h);
           paged_read_scales<cur * 2 * C::KB * 4 + C::KB * 4 + mb * 128>(sv, lds0 + C::SCALES + 16 * h);
         }
-        f32x16_t sc[RB];
+        f32x16_t s;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sc[rb][r] = 0.f;
-        static_for<KS>([&](auto sc_) {
-          constexpr int st = decltype(sc_)::value;
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        static_for<KS>([&](auto stc) {
+          constexpr int st = decltype(stc)::value;
           u32x4_t a;
           if constexpr (FP8) a = paged_codes_to_bf16(kf[st / 2][2 * (st % 2)], kf[st / 2][2 * (st % 2) + 1]);
           else a = kf[st];
-#pragma unroll
-          for (int rb = 0; rb < RB; ++rb) sc[rb] = attn_mfma(a, __builtin_bit_cast(u32x4_t, qf[rb][st]), sc[rb]);
+          s = attn_mfma(a, __builtin_bit_cast(u32x4_t, qf[st]), s);
         });
         __builtin_amdgcn_sched_barrier(0);
         paged_read_columns<C::RBY, base + C::TILE + mb * 32 * C::RBY>(vq, L.tr);
+        if constexpr (FP8) {
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          if constexpr (FP8) {
+          for (int r = 0; r < 16; ++r) s[r] *= __uint_as_float(sk[r >> 2][r & 3]);
+        }
+        const int k32 = kb + 32 * mb;
+        if (k32 + 32 > W.all_see) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[rb][r] *= __uint_as_float(sk[r >> 2][r & 3]);
-          }
-          const int k32 = kb + 32 * mb;
-          if (k32 + 32 > W.all_see) {
+          for (int r = 0; r < 16; ++r) s[r] = k32 + 4 * h + 8 * (r >> 2) + (r & 3) < seen ? s[r] : -INFINITY;
+        }
+        float mx = -INFINITY, mlo, mhi;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[rb][r] = k32 + 4 * h + 8 * (r >> 2) + (r & 3) < seen[rb] ? sc[rb][r] : -INFINITY;
-          }
-          float mx = -INFINITY;
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        attn_halves(mx, mlo, mhi);
+        const float m_new = fmaxf(m_run, fmaxf(mlo, mhi) * c), m_use = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m_run - m_use);
+        float sum[2] = {0.f, 0.f};
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[rb][r]);
-          float mlo, mhi;
-          attn_halves(mx, mlo, mhi);
-          const float m_new = fmaxf(m_run[rb], fmaxf(mlo, mhi) * c), m_use = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m_run[rb] - m_use);
-          float sum[2] = {0.f, 0.f};
+        for (int r = 0; r < 16; ++r) {
+          const float e = fast_exp2(__builtin_fmaf(s[r], c, -m_use));
+          sum[r & 1] += e;
+          s[r] = FP8 ? e * __uint_as_float(sv[r >> 2][r & 3]) : e;
+        }
+        l_run = l_run * alpha + (sum[0] + sum[1]);
+        m_run = m_new;
+        if (__any(alpha != 1.f)) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float e = fast_exp2(__builtin_fmaf(sc[rb][r], c, -m_use));
-            sum[r & 1] += e;
-            sc[rb][r] = FP8 ? e * __uint_as_float(sv[r >> 2][r & 3]) : e;
-          }
-          l_run[rb] = l_run[rb] * alpha + (sum[0] + sum[1]);
-          m_run[rb] = m_new;
-          if (__any(alpha != 1.f)) {
+          for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) acc[rb][db][r] *= alpha;
-          }
+            for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
         }
         __builtin_amdgcn_sched_barrier(0);
         static_for<2>([&](auto qc) {
           constexpr int q = decltype(qc)::value;
-          u32x4_t pf[RB];
+          float tmp[8];
 #pragma unroll
-          for (int rb = 0; rb < RB; ++rb) {
-            float tmp[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) tmp[j] = sc[rb][8 * q + j];
-            pf[rb] = __builtin_bit_cast(u32x4_t, attn_pack8(tmp));
-          }
+          for (int j = 0; j < 8; ++j) tmp[j] = s[8 * q + j];
+          const u32x4_t pf = __builtin_bit_cast(u32x4_t, attn_pack8(tmp));
           static_for<VB>([&](auto nc) {
             constexpr int n = decltype(nc)::value;
             const u32x4_t v = {vq[q][n].lo.x, vq[q][n].lo.y, vq[q][n].hi.x, vq[q][n].hi.y};
@@ -551,13 +531,10 @@ static __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttn p, Page
 #pragma unroll
               for (int odd = 0; odd < 2; ++odd) {
                 const uint32_t sel = odd ? 0x07050301u : 0x06040200u;
-                const u32x4_t a = paged_codes_to_bf16(__builtin_amdgcn_perm(v[1], v[0], sel), __builtin_amdgcn_perm(v[3], v[2], sel));
-#pragma unroll
-                for (int rb = 0; rb < RB; ++rb) acc[rb][2 * n + odd] = attn_mfma(a, pf[rb], acc[rb][2 * n + odd]);
+                acc[2 * n + odd] = attn_mfma(paged_codes_to_bf16(__builtin_amdgcn_perm(v[1], v[0], sel), __builtin_amdgcn_perm(v[3], v[2], sel)), pf, acc[2 * n + odd]);
               }
             } else {
-#pragma unroll
-              for (int rb = 0; rb < RB; ++rb) acc[rb][n] = attn_mfma(v, pf[rb], acc[rb][n]);
+              acc[n] = attn_mfma(v, pf, acc[n]);
             }
           });
           __builtin_amdgcn_sched_barrier(0);
@@ -570,20 +547,16 @@ static __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttn p, Page
         if (kb + i * C::KB < W.k1) step(ic, kb + i * C::KB);
       });
     FGRPO_WAIT_VMCNT(0);         // the loads behind the stretch: the next one's go to the same buffers
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      float l_lo, l_hi;
-      attn_halves(l_run[rb], l_lo, l_hi);
-      const float l = l_lo + l_hi;
-      const int row = W.r0 + 32 * rb + (lane & 31), tok = W.q0 + row / p.G, hq = W.head * p.G + row % p.G;
-      if (row >= W.rows) continue;
-      if (W.begins && W.ends) {
-        paged_store_row<HD, FP8>(acc[rb], l > 0.f ? 1.f / l : 0.f, p.out + ((long long)tok * p.Hq + hq) * HD, h);
-        if (p.lse && h == 0) p.lse[(long long)hq * p.c.T + tok] = paged_lse(m_run[rb], l);
-      } else {
-        attn_store_partial(acc[rb], sp.part + ((long long)W.slot() * RB + rb) * (32 * HD), lane);
-        if (h == 0) sp.ml[((long long)W.slot() * RB + rb) * 32 + lane] = make_float2(m_run[rb], l);
-      }
+    float l_lo, l_hi;
+    attn_halves(l_run, l_lo, l_hi);
+    const float l = l_lo + l_hi;
+    if (W.r0 + (lane & 31) >= W.rows) return;
+    if (W.begins && W.ends) {
+      paged_store_row<HD, FP8>(acc, l > 0.f ? 1.f / l : 0.f, p.out + ((long long)(W.q0 + tok) * p.Hq + hq) * HD, h);
+      if (p.lse && h == 0) p.lse[(long long)hq * p.c.T + W.q0 + tok] = paged_lse(m_run, l);
+    } else {
+      attn_store_partial(acc, sp.part + (long long)W.slot() * (32 * HD), lane);
+      if (h == 0) sp.ml[(long long)W.slot() * 32 + lane] = make_float2(m_run, l);
     }
   });
 }
