@@ -62,7 +62,7 @@ struct PagedPlan {
   int rows, W, items;      // items: as in PagedSplit
   int shape() const { return rows == 16 ? 16 : 32; }
   size_t slots() const { return 2ull * W; }
-  size_t rec_bytes() const { return slots() * 2 * sizeof(int4); }
+  size_t rec_bytes() const { return (size_t)W * 2 * sizeof(int4); }
   size_t part_bytes(int D) const { return slots() * rows * D * 4; }
   size_t bytes(int D) const { return rec_bytes() + part_bytes(D) + slots() * rows * sizeof(float2); }
 };
@@ -82,7 +82,7 @@ int launch_merge(const PagedAttn& p, const PagedSplit& sp, hipStream_t st) {
   if (sp.items > 0)
     hipLaunchKernelGGL((paged_merge_items_kernel<HD, PAIRS, SHAPE, RB>), dim3(sp.items, RB * HD / (SHAPE == 32 ? 8 : 16)), dim3(256), 0, st, p, sp);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<HD, PAIRS, SHAPE, RB>), dim3(sp.odd ? sp.W : 2 * sp.W, RB), dim3(256), 0, st, p, sp);
+    hipLaunchKernelGGL((paged_merge_kernel<HD, PAIRS, SHAPE, RB>), dim3(sp.W, RB), dim3(256), 0, st, p, sp);
   HIP_TRY(hipGetLastError());
   return 0;
 }
@@ -174,7 +174,7 @@ int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride
   if (!ws || ws_bytes < need) return fail(FGRPO_ERR_WORKSPACE, "paged_attn_fwd: workspace %zu < %zu", ws ? ws_bytes : 0, need);
   if (!aligned16(ws)) return fail(FGRPO_ERR_ALIGN, "paged_attn_fwd: workspace must be 16-byte aligned");
   PagedSplit sp;
-  sp.W = plan.W, sp.odd = plan.rows != kPagedRows, sp.items = plan.items, sp.most_parts = plan.items > 0 ? 1024 : 128;      // what a merge reads one behind the other
+  sp.W = plan.W, sp.items = plan.items, sp.most_parts = plan.items > 0 ? 1024 : 128;      // what a merge reads one behind the other
   sp.rec = (int4*)ws;
   sp.part = (float*)((char*)ws + plan.rec_bytes());
   sp.ml = (float2*)((char*)sp.part + plan.part_bytes(cache->head_dim));

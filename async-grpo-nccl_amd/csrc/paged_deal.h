@@ -13,13 +13,12 @@ namespace fgrpo {
 
 struct PagedSplit {
   int W;                 // work-groups of the launch, a multiple of 8
-  int odd;               // only odd slots begin items (shares alone)
-  int items;             // > 0: no more items than this, few enough for the merge to have work-groups for every unit of each: records go by item, not by slot
+  int items;             // > 0: no more items than this, few enough for the merge to have work-groups for every unit of each: records go by item, not by work-group
   int most_parts;        // of an item
   float* part;           // [2 W][row blocks][units][64 lanes][4] sums of a part (paged_column)
   float2* ml;            // [2 W][rows] maximum (in powers of two) and sum
-  int4* rec;             // [2 W][2] for the slot of an item's first part, what its merge needs: {parts (0: none; negative: their slots are neighbours), first
-                         // packed row of the sequence, first row of the tile, rows of the sequence}, {head, its slot}
+  int4* rec;             // [W][2] what the merge of an item needs, for each that a work-group begins and does not end: {parts (0: none; negative: their slots
+                         // are neighbours), first packed row of the sequence, first row of the tile, rows of the sequence}, {head, slot of the first part}
 };
 // slot of part i of an item whose first is in `slot`.  Shares: work-group w has 2 w for an item that an earlier one began and 2 w + 1 for one
 // that it begins and does not end.
@@ -33,12 +32,18 @@ struct PagedWeight {
   __device__ __forceinline__ double of(int t) const { return base + slope * (t + 1); }
   __device__ __forceinline__ double upto(int n) const { return base * n + slope * 0.5 * n * (n + 1.0); }      // tiles 0 .. n - 1
 };
+// A parameter as if it were read here: what is made of it (its double, above all) is not carried in registers across the loops between its uses
+__device__ __forceinline__ int at_hand(int x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
 template <int ROWS>
 __device__ __forceinline__ PagedWeight paged_weight(const PagedAttn& p, int q0, int nq, int len) {
   PagedWeight w;
   w.q0 = q0, w.nq = nq, w.len = len;
-  w.tiles = (int)(((long long)nq * p.G + ROWS - 1) / ROWS);
-  w.base = (double)(p.causal ? max(len - nq, 0) : len) * p.G + ROWS;
+  const int G = at_hand(p.G);
+  w.tiles = (int)(((long long)nq * G + ROWS - 1) / ROWS);
+  w.base = (double)(p.causal ? max(len - nq, 0) : len) * G + ROWS;
   w.slope = p.causal ? ROWS : 0;
   return w;
 }
@@ -112,12 +117,13 @@ struct PagedItem {
 // The item that holds place `x` of the weights, or of the numbers.
 template <int ROWS, bool NUMBERS>
 __device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, PagedLanes<ROWS>& lanes, double x) {
+  const int Hkv = at_hand(p.c.Hkv);
   PagedItem s{p.c.B, 0, 0, 0, 0};
   double weight = 0, number = 0;      // in front of the 64 at hand
   for (int b0 = 0; b0 < p.c.B; b0 += 64) {
     if (lanes.b0 != b0) lanes.load(p, b0);
     const PagedWeight w = lanes.mine(p);
-    const double m = w.upto(w.tiles) * p.c.Hkv, n = (double)w.tiles * p.c.Hkv, upto_m = wave_sums(m), upto_n = wave_sums(n);
+    const double m = w.upto(w.tiles) * Hkv, n = (double)w.tiles * Hkv, upto_m = wave_sums(m), upto_n = wave_sums(n);
     const unsigned long long past = __ballot((NUMBERS ? number + upto_n : weight + upto_m) > x);      // the first lane past it holds the sequence
     if (past) {
       const int at = __ffsll(past) - 1;
@@ -132,9 +138,9 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, PagedLanes<R
   const PagedWeight w = lanes.of(p, s.b);
   const double one = NUMBERS ? (double)w.tiles : w.upto(w.tiles);      // of one head
   double r = x - (NUMBERS ? s.index : s.at);
-  int head = (int)fmin(floor(r / one), p.c.Hkv - 1.0), t = 0;
+  int head = (int)fmin(floor(r / one), Hkv - 1.0), t = 0;
   if (head > 0 && one * head > r) --head;
-  if (head + 1 < p.c.Hkv && one * (head + 1) <= r) ++head;
+  if (head + 1 < Hkv && one * (head + 1) <= r) ++head;
   r -= one * head;
   if (NUMBERS) {
     t = (int)fmin(r, w.tiles - 1.0);
@@ -284,19 +290,18 @@ static __global__ __launch_bounds__(256) void paged_merge_items_kernel(PagedAttn
   if (p.lse && unit == 0 && lane < SHAPE) p.lse[(long long)hq * p.c.T + tok] = paged_lse(sum.m, sum.l);
 }
 
-// Adds up the parts of the item whose first is in slot blockIdx.x (2 blockIdx.x + 1: only odd ones begin items), in the order of the keys: work-group y takes
-// block y of SHAPE rows, wavefront w the units w, w + 4 .. of their columns.  RB: blocks of a tile.
+// Adds up the parts of the item of record blockIdx.x in the order of the keys: work-group y takes block y of SHAPE rows, wavefront w the units w, w + 4 ..
+// of their columns.  RB: blocks of a tile.
 template <int HD, bool PAIRS, int SHAPE, int RB>
 static __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p, PagedSplit sp) {
   constexpr int NU = HD / (SHAPE == 32 ? 8 : 16) / 4, WIDE = 16 / NU < 8 ? 16 / NU : 8;
-  const int first = sp.odd ? 2 * blockIdx.x + 1 : blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rb = blockIdx.y;
-  const int4 rec = sp.rec[2 * first];
-  const int head = sp.rec[2 * first + 1].x;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rb = blockIdx.y;
+  const int4 rec = sp.rec[2 * blockIdx.x], place = sp.rec[2 * blockIdx.x + 1];
   if (rec.x == 0) return;
   const bool neighbours = rec.x < 0;
   const int np = neighbours ? -rec.x : rec.x, row = rec.z + SHAPE * rb + lane % SHAPE;
   if (row >= rec.w) return;
-  const int tok = rec.y + row / p.G, hq = head * p.G + row % p.G;
+  const int tok = rec.y + row / p.G, hq = place.x * p.G + row % p.G;
   PagedSum sum[NU];
 #pragma unroll
   for (int c = 0; c < NU; ++c) sum[c] = PagedSum{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
@@ -307,7 +312,7 @@ static __global__ __launch_bounds__(256) void paged_merge_kernel(PagedAttn p, Pa
     float4 y[WIDE][NU];
 #pragma unroll
     for (int i = 0; i < WIDE; ++i) {
-      const long long slot = (long long)RB * min(paged_slot(first, min(i0 + i, np - 1), neighbours), 2 * sp.W - 1);
+      const long long slot = (long long)RB * min(paged_slot(place.y, min(i0 + i, np - 1), neighbours), 2 * sp.W - 1);
       x[i] = ml[slot * SHAPE];
 #pragma unroll
       for (int c = 0; c < NU; ++c) y[i][c] = *(const float4*)(part + slot * (SHAPE * HD) + 1024 * c);

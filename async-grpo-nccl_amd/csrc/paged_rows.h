@@ -279,7 +279,7 @@ struct PagedWalk {
       if (w == 0)
         for (int i = (int)total.items + lane; i < sp.items; i += 64) sp.rec[2 * i] = make_int4(0, 0, 0, 0);      // there are no more
     } else if (lane == 0) {
-      sp.rec[4 * w + 2] = rec, sp.rec[4 * w + 3] = make_int4(rec_head, 2 * w + 1, 0, 0);      // slot 2 w + 1: only odd slots are looked at
+      sp.rec[2 * w] = rec, sp.rec[2 * w + 1] = make_int4(rec_head, 2 * w + 1, 0, 0);
     }
   }
 };

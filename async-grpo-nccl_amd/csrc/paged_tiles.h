@@ -23,6 +23,8 @@ template <int HD, bool FP8>
 struct PagedTiles {
   static constexpr int ES = FP8 ? 1 : 2, RBY = HD * ES, TILE = kAttnBK * HD * 2, BUF = 2 * TILE;
   static constexpr int CPR = RBY / 16, RPI = 1024 / RBY, IPG = 16 / RPI;      // as the cache has its rows: 16-byte chunks, rows and instructions of 16 keys
+  // e4m3: rows that share banks under the swizzle trade neighbouring chunks, as the lanes of a write hold every other chunk of two of them
+  static __device__ __forceinline__ int odd(int row) { return HD == 128 ? row & 1 : (row >> 1) & 1; }
   static constexpr int T0 = FP8 ? 4 * kAttnBK * 4 : 0, LDS = T0 + 2 * BUF;      // the scales of both buffers lie in front (K, then V)
 };
 
@@ -51,6 +53,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
   {
     const AttnLane<HD> L = attn_lane<HD>(lane);
     row_at = L.rowc[0] + lds0 + C::T0, tr_at[0] = L.tr[0][0] + lds0 + C::T0, tr_at[1] = L.tr[0][1] + lds0 + C::T0;
+    if constexpr (FP8) row_at ^= C::odd(lane & 31) << 4, tr_at[0] ^= C::odd((lane & 15) >> 2) << 4, tr_at[1] ^= C::odd((lane & 15) >> 2) << 4;
   }
   auto anew = [](uint32_t x) {      // formed at each use: e4m3 has no registers to carry all of them
     if constexpr (FP8) asm volatile("" : "+v"(x));
@@ -61,7 +64,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
   // the swizzle that i decides; and, codes, where they write (of 16 codes the first eight; the others and other i flip bits)
   const int row16 = lane / C::CPR, at16 = 16 * wave + row16, ch = FP8 ? lane % C::CPR : (lane % C::CPR) ^ attn_swz<HD>(at16);
   const uint32_t voff_k = (uint32_t)(row16 * p.c.k_st[1] * C::ES), voff_v = (uint32_t)(row16 * p.c.v_st[1] * C::ES);
-  const uint32_t put = lds0 + C::T0 + at16 * (HD * 2) + (((2 * ch) ^ attn_swz<HD>(at16)) << 4);
+  const uint32_t put = lds0 + C::T0 + at16 * (HD * 2) + (((2 * ch) ^ attn_swz<HD>(at16) ^ C::odd(at16)) << 4);
   auto flip = [](int i) { return attn_swz<HD>(i * C::RPI); };      // the swizzle of row16 + i RPI is that of row16 with these bits flipped: RPI is a power of two above row16
 
   // x0 .. x1 of an item's weight; whole: its output, else sums for `slot`
@@ -195,13 +198,20 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
             s2[g / 2] = attn_mfma(kf[g % 2][i], __builtin_bit_cast(u32x4_t, qf[G4 * (g % 2) + i]), s2[g / 2]);
           }
         };
-        // scales of the 32 keys of a half, four instructions' worth
-        auto scale_by = [&](auto mbc, auto which) {
+        u32x4_t sk[4];              // scales of the 32 keys of a half, of K and then of V
+        auto req_scales = [&](auto mbc, auto which) {
           constexpr int mb = decltype(mbc)::value;
-          u32x4_t f[4];
-          paged_read_scales<cur * 2 * kAttnBK * 4 + decltype(which)::value * kAttnBK * 4 + mb * 128>(f, lds0 + 16 * h);
+          static_for<4>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            sk[i] = lds_read_u128_asm<cur * 2 * kAttnBK * 4 + decltype(which)::value * kAttnBK * 4 + mb * 128 + 32 * i>(lds0 + 16 * h);
+          });
+        };
+        auto scale_half = [&](auto mbc) {
+          constexpr int mb = decltype(mbc)::value;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s2[mb][r] *= __uint_as_float(f[r >> 2][r & 3]);
+          for (int i = 0; i < 4; ++i) attn_settle(sk[i]);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s2[mb][r] *= __uint_as_float(sk[r >> 2][r & 3]);
         };
         req_k(I0{});
         req_k(I1{});
@@ -220,11 +230,23 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
         __builtin_amdgcn_sched_barrier(0);
         mma_k(I2{});
         __builtin_amdgcn_sched_barrier(0);
-        wait_lgkm<2 * DB>();
+        if constexpr (FP8) req_scales(I0{}, I0{});
+        wait_lgkm<2 * DB + (FP8 ? 4 : 0)>();
         __builtin_amdgcn_sched_barrier(0);
         mma_k(I3{});
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (FP8) scale_by(I0{}, I0{}), scale_by(I1{}, I0{});
+        if constexpr (FP8) {
+          wait_lgkm<0>();
+          __builtin_amdgcn_sched_barrier(0);
+          scale_half(I0{});
+          __builtin_amdgcn_sched_barrier(0);
+          req_scales(I1{}, I0{});
+          wait_lgkm<0>();
+          __builtin_amdgcn_sched_barrier(0);
+          scale_half(I1{});
+          __builtin_amdgcn_sched_barrier(0);
+          req_scales(I0{}, I1{});
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb) {
@@ -261,10 +283,17 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
         }
-        if constexpr (FP8) scale_by(I0{}, I1{}), scale_by(I1{}, I1{});
+        if constexpr (FP8) {
+          wait_lgkm<0>();
+          __builtin_amdgcn_sched_barrier(0);
+          scale_half(I0{});
+          __builtin_amdgcn_sched_barrier(0);
+          req_scales(I1{}, I1{});      // lands with the next group's columns
+        }
         __builtin_amdgcn_sched_barrier(0);
         static_for<4>([&](auto qc) {
           constexpr int q = decltype(qc)::value, mb = q / 2, half = q % 2;
+          if constexpr (FP8 && q == 2) scale_half(I1{});
           if constexpr (q < 3) req_v(std::integral_constant<int, q + 1>{});
           wait_lgkm<(q < 3 ? 2 * DB : 0)>();
           __builtin_amdgcn_sched_barrier(0);
@@ -311,17 +340,17 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
   int first = 0, rounds = 0, left = 0, parts = 1, turn = 0;      // whole items: the XCD's first, rounds of n, those of the last round, their parts; this work-group's turn
   PagedItem s{0, 0, 0, 0, 0};
   if (shares) {
-    if (threadIdx.x == 0) sp.rec[4 * w] = sp.rec[4 * w + 2] = none;
+    if (threadIdx.x == 0) sp.rec[2 * w] = none;
     if (!(w < sh.used)) return;
     done = sh.bound(w), hi = sh.bound(w + 1);
     if (!(done < hi)) return;
     s = paged_item<ROWS, false>(p, lanes, done);
   } else {                       // those that begin in this XCD's eighth of the weights
-    if (threadIdx.x == 0) sp.rec[2 * (2 * n * xcd + me)] = sp.rec[2 * (2 * n * xcd + n + me)] = none;
     first = __builtin_amdgcn_readfirstlane((int)paged_item<ROWS, false>(p, lanes, floor(total.weight * xcd / 8)).index);
     const int last = xcd == 7 ? (int)total.items : (int)paged_item<ROWS, false>(p, lanes, floor(total.weight * (xcd + 1) / 8)).index;
     const int items = __builtin_amdgcn_readfirstlane(last) - first;
     rounds = items / n, left = items - rounds * n, parts = __builtin_amdgcn_readfirstlane(paged_last_parts(left, n));
+    if (threadIdx.x == 0 && (me >= left || parts == 1)) sp.rec[2 * w] = none;      // record `me` of the XCD is its item `me` of the last round's
   }
   if (threadIdx.x == 0) kept[0] = sh.total, kept[1] = sh.used, kept[2] = hi;      // what the walks must not carry in registers
   __syncthreads();
@@ -353,7 +382,10 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     } else {
       x1 = weight;
     }
-    if (rec != 0 && threadIdx.x == 0) sp.rec[2 * slot] = make_int4(rec, wt.q0, s.t * ROWS, wt.nq * p.G), sp.rec[2 * slot + 1] = make_int4(s.head, slot, 0, 0);
+    if (rec != 0 && threadIdx.x == 0) {
+      const int at = shares ? w : n * xcd + (slot - 2 * n * xcd) / parts;
+      sp.rec[2 * at] = make_int4(rec, wt.q0, s.t * ROWS, wt.nq * p.G), sp.rec[2 * at + 1] = make_int4(s.head, slot, 0, 0);
+    }
     walk(s, wt, x0, x1, slot);
     lanes.b0 = -64;            // read again, as these are
     sh.total = uniform(kept[0]), sh.used = uniform(kept[1]), hi = uniform(kept[2]);

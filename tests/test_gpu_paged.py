@@ -109,6 +109,20 @@ def test_attention_over_the_cache(dev, shape, Hq, Hkv, D, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D,qs,ks", [
+    # as many tiles as work-groups and a few: whole ones in rounds, the rest in parts
+    (12, 2, 128, [700, 690, 711, 705, 650, 730, 700, 680], [1000, 1100, 711, 1205, 650, 900, 1000, 980]),
+    # one long sequence among short ones: shares
+    (14, 2, 64, [1, 900, 3, 1, 40], [700, 1500, 64, 1, 2000]),
+    # a prompt from its start, rows from one key to all
+    (8, 1, 128, [1500], [1500])])
+def test_attention_of_many_tiles(dev, Hq, Hkv, D, qs, ks, fp8):
+    s = _batch(qs, ks, Hq, Hkv, D, 64, fp8, seed=3)
+    out, lse = ops.paged_attention(s["q"].to(dev), _cache(s, dev), s["table"].to(dev), s["lens"].to(dev), s["cu"].to(dev), max_len=max(qs), return_lse=True)
+    _check(s, out, lse)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("D", [128, 64])
 def test_write_then_read(dev, D, fp8):
     Hkv, block = 3, 32
