@@ -155,11 +155,11 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, PagedLanes<R
   s.at = uniform(s.at + w.upto(w.tiles) * s.head + w.upto(s.t)), s.index = uniform(s.index + (double)w.tiles * s.head + s.t);
   return s;
 }
+// The next item; s.at already is where it begins.
 template <int ROWS>
 __device__ __forceinline__ void paged_next(const PagedAttn& p, PagedLanes<ROWS>& lanes, PagedItem& s) {
-  const PagedWeight w = lanes.of(p, s.b);
-  s.at = uniform(s.at + w.of(s.t)), s.index = uniform(s.index + 1);
-  if (++s.t < w.tiles) return;
+  s.index = uniform(s.index + 1);
+  if (++s.t < lanes.of(p, s.b).tiles) return;
   s.t = 0;
   if (++s.head < p.c.Hkv) return;
   s.head = 0;

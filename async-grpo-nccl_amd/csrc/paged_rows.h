@@ -270,7 +270,7 @@ struct PagedWalk {
       }
       look_up(k0);
       item();
-      done = uniform(s.at + weight);
+      s.at = done = uniform(s.at + weight);
       if (done >= hi) break;
       paged_next<ROWS>(p, lanes, s);
       if (s.b >= p.c.B) break;

@@ -21,12 +21,24 @@ constexpr int kPagedTileRB = kPagedRows / 32;
 
 template <int HD, bool FP8>
 struct PagedTiles {
-  static constexpr int ES = FP8 ? 1 : 2, RBY = HD * ES, TILE = kAttnBK * HD * 2, BUF = 2 * TILE;
+  static constexpr int ES = FP8 ? 1 : 2, RBY = HD * ES;
   static constexpr int CPR = RBY / 16, RPI = 1024 / RBY, IPG = 16 / RPI;      // as the cache has its rows: 16-byte chunks, rows and instructions of 16 keys
-  // e4m3: rows that share banks under the swizzle trade neighbouring chunks, as the lanes of a write hold every other chunk of two of them
-  static __device__ __forceinline__ int odd(int row) { return HD == 128 ? row & 1 : (row >> 1) & 1; }
+  // Rows of the tiles in LDS.  What the direct loads write has no room between rows: chunks are swizzled (attn_swz).  What comes through registers has:
+  // rows 16 bytes apart do not share banks where 16 of them are read at one chunk, rows 64 bytes apart where 4 are at 64 bytes, and every
+  // fragment address is one register and a constant.
+  static constexpr int KROW = HD * 2 + (FP8 ? 16 : 0), VROW = HD * 2 + (FP8 ? 64 : 0);
+  static constexpr int KTILE = kAttnBK * KROW, BUF = KTILE + kAttnBK * VROW;
   static constexpr int T0 = FP8 ? 4 * kAttnBK * 4 : 0, LDS = T0 + 2 * BUF;      // the scales of both buffers lie in front (K, then V)
 };
+
+template <int OFF0, int OFF1>
+__device__ __forceinline__ AttnTr paged_rd_tr(uint32_t a) {      // attn_rd_tr_asm from one address
+  static_assert(OFF1 < 65536, "DS offset field");
+  AttnTr f;
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.lo) : "v"(a), "i"(OFF0));
+  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.hi) : "v"(a), "i"(OFF1));
+  return f;
+}
 
 // Parts of the last, incomplete round of `left` items on `n` work-groups: the shortest of rounds / parts, a cut costing about a 20th of an item.
 __device__ __forceinline__ int paged_last_parts(int left, int n) {
@@ -44,27 +56,25 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
   using C = PagedTiles<HD, FP8>;
   constexpr int KS = HD / 16, DB = HD / 32, G4 = KS / 2, ROWS = kPagedRows;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];      // fragment addresses are formed by flipping bits below 1024
-  __shared__ double kept[3];
+  __shared__ double kept[5];
   const uint32_t lds0 = lds_addr(smem);
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int xcd = blockIdx.x & 7, n = sp.W >> 3, me = blockIdx.x >> 3, w = xcd * n + me;
-  // fragment addresses: of k step st the row's first with bits of its chunk flipped, of column block db likewise (AttnLane)
+  // fragment addresses.  bf16: of k step st the row's first with bits of its chunk flipped, of column block db likewise (AttnLane); e4m3: of buffer 0
   uint32_t row_at, tr_at[2];
-  {
+  if constexpr (FP8) {
+    row_at = lds0 + C::T0 + (lane & 31) * C::KROW + h * 16;
+    tr_at[0] = lds0 + C::T0 + C::KTILE + (4 * h + ((lane & 15) >> 2)) * C::VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8, tr_at[1] = 0;
+  } else {
     const AttnLane<HD> L = attn_lane<HD>(lane);
-    row_at = L.rowc[0] + lds0 + C::T0, tr_at[0] = L.tr[0][0] + lds0 + C::T0, tr_at[1] = L.tr[0][1] + lds0 + C::T0;
-    if constexpr (FP8) row_at ^= C::odd(lane & 31) << 4, tr_at[0] ^= C::odd((lane & 15) >> 2) << 4, tr_at[1] ^= C::odd((lane & 15) >> 2) << 4;
+    row_at = L.rowc[0] + lds0, tr_at[0] = L.tr[0][0] + lds0, tr_at[1] = L.tr[0][1] + lds0;
   }
-  auto anew = [](uint32_t x) {      // formed at each use: e4m3 has no registers to carry all of them
-    if constexpr (FP8) asm volatile("" : "+v"(x));
-    return x;
-  };
   const float c = p.scale * kLog2e;
   // where this wavefront's lanes read: row lane / CPR of 16 and every RPI-th behind it, and of instruction i chunk `ch`, but for the bits of
-  // the swizzle that i decides; and, codes, where they write (of 16 codes the first eight; the others and other i flip bits)
+  // the swizzle that i decides; and, codes, where they write
   const int row16 = lane / C::CPR, at16 = 16 * wave + row16, ch = FP8 ? lane % C::CPR : (lane % C::CPR) ^ attn_swz<HD>(at16);
   const uint32_t voff_k = (uint32_t)(row16 * p.c.k_st[1] * C::ES), voff_v = (uint32_t)(row16 * p.c.v_st[1] * C::ES);
-  const uint32_t put = lds0 + C::T0 + at16 * (HD * 2) + (((2 * ch) ^ attn_swz<HD>(at16) ^ C::odd(at16)) << 4);
+  const uint32_t put_k = lds0 + C::T0 + at16 * C::KROW + ch * 32, put_v = lds0 + C::T0 + C::KTILE + at16 * C::VROW + ch * 32;
   auto flip = [](int i) { return attn_swz<HD>(i * C::RPI); };      // the swizzle of row16 + i RPI is that of row16 with these bits flipped: RPI is a power of two above row16
 
   // x0 .. x1 of an item's weight; whole: its output, else sums for `slot`
@@ -105,7 +115,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
 #pragma unroll
         for (int i = 0; i < C::IPG; ++i) {
           __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, FGRPO_LDS_PTR(t + i * 1024), 16, (int)(voff_k + (ch ^ flip(i)) * 16), (int)(i * C::RPI * p.c.k_st[1] * 2), 0, 0);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, FGRPO_LDS_PTR(t + C::TILE + i * 1024), 16, (int)(voff_v + (ch ^ flip(i)) * 16), (int)(i * C::RPI * p.c.v_st[1] * 2), 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, FGRPO_LDS_PTR(t + C::KTILE + i * 1024), 16, (int)(voff_v + (ch ^ flip(i)) * 16), (int)(i * C::RPI * p.c.v_st[1] * 2), 0, 0);
         }
       }
       look_up(kb + kAttnBK);
@@ -113,14 +123,14 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     auto put_codes = [&](auto bufc) {      // registers -> LDS, as bf16
       constexpr int buf = decltype(bufc)::value;
       if constexpr (FP8) {
-#pragma unroll
-        for (int i = 0; i < C::IPG; ++i)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t at = (put ^ ((u ^ flip(i)) << 4)) + i * C::RPI * (HD * 2);
-            lds_write_u128_asm<buf * C::BUF>(at, paged_codes_to_bf16(raw[2 * i][2 * u], raw[2 * i][2 * u + 1]));
-            lds_write_u128_asm<buf * C::BUF + C::TILE>(at, paged_codes_to_bf16(raw[2 * i + 1][2 * u], raw[2 * i + 1][2 * u + 1]));
-          }
+        static_for<C::IPG>([&](auto ic) {
+          constexpr int i = decltype(ic)::value;
+          static_for<2>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            lds_write_u128_asm<i * C::RPI * C::KROW + u * 16>(put_k + buf * C::BUF, paged_codes_to_bf16(raw[2 * i][2 * u], raw[2 * i][2 * u + 1]));
+            lds_write_u128_asm<i * C::RPI * C::VROW + u * 16>(put_v + buf * C::BUF, paged_codes_to_bf16(raw[2 * i + 1][2 * u], raw[2 * i + 1][2 * u + 1]));
+          });
+        });
         if (lane < 16) {
           lds_write_u32_asm<buf * 2 * kAttnBK * 4>(lds0 + (16 * wave + lane) * 4, raw_scale[0]);
           lds_write_u32_asm<buf * 2 * kAttnBK * 4 + kAttnBK * 4>(lds0 + (16 * wave + lane) * 4, raw_scale[1]);
@@ -153,11 +163,11 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
       if (k0 + kAttnBK < k1) fetch(0, k0 + kAttnBK);
       wait_lgkm<0>();
     } else {
-      FGRPO_WAIT_VMCNT(0);
+      FGRPO_WAIT_VMCNT_LGKM0(0);
     }
     wg_barrier();
     auto step = [&](auto curc, int kb) {
-      constexpr int cur = decltype(curc)::value, kt = cur * C::BUF, vt = kt + C::TILE;
+      constexpr int cur = decltype(curc)::value, kt = cur * C::BUF, vt = kt + C::KTILE;
       if (kb + kAttnBK < k1) {
         if constexpr (FP8) {
           put_codes(std::integral_constant<int, cur ^ 1>{});
@@ -176,18 +186,18 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
           for (int r = 0; r < 16; ++r) s2[mb][r] = 0.f;
         auto req_k = [&](auto gc) {
           constexpr int g = decltype(gc)::value;
-          const uint32_t at = anew(row_at);
           static_for<G4>([&](auto ic) {
             constexpr int i = decltype(ic)::value, st = G4 * (g % 2) + i;
-            kf[g % 2][i] = lds_read_u128_asm<kt + (g / 2) * 32 * HD * 2>(at ^ (st << 5));
+            if constexpr (FP8) kf[g % 2][i] = lds_read_u128_asm<(g / 2) * 32 * C::KROW + st * 32>(row_at + kt);
+            else kf[g % 2][i] = lds_read_u128_asm<kt + (g / 2) * 32 * C::KROW>(row_at ^ (st << 5));
           });
         };
         auto req_v = [&](auto qc) {
           constexpr int q = decltype(qc)::value;
-          const uint32_t lo = anew(tr_at[0]), hi = anew(tr_at[1]);
           static_for<DB>([&](auto dc) {
             constexpr int db = decltype(dc)::value;
-            vq[q % 2][db] = attn_rd_tr_asm<vt + 16 * q * HD * 2>(lo ^ (db << 6), hi ^ (db << 6));
+            if constexpr (FP8) vq[q % 2][db] = paged_rd_tr<16 * q * C::VROW + db * 64, 16 * q * C::VROW + db * 64 + 8 * C::VROW>(tr_at[0] + kt);
+            else vq[q % 2][db] = attn_rd_tr_asm<vt + 16 * q * C::VROW>(tr_at[0] ^ (db << 6), tr_at[1] ^ (db << 6));
           });
         };
         auto mma_k = [&](auto gc) {
@@ -366,7 +376,6 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
         s = paged_item<ROWS, true>(p, lanes, first + rounds * n + i / parts);
         slot = 2 * n * xcd + i, part = i % parts;
       }
-      ++turn;
     }
     if (s.b >= p.c.B) break;
     const PagedWeight wt = lanes.of(p, s.b);
@@ -376,7 +385,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
       x0 = done - s.at, x1 = fmin(hi - s.at, weight);
       slot = 2 * w + (x0 <= 0);
       if (x0 <= 0 && x1 < weight) rec = sh.holding(s.at + weight - 1) - w + 1;
-    } else if (turn > rounds) {
+    } else if (turn >= rounds) {
       x0 = floor(weight * part / parts), x1 = floor(weight * (part + 1) / parts);
       if (parts > 1 && part == 0) rec = -parts;
     } else {
@@ -386,11 +395,13 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
       const int at = shares ? w : n * xcd + (slot - 2 * n * xcd) / parts;
       sp.rec[2 * at] = make_int4(rec, wt.q0, s.t * ROWS, wt.nq * p.G), sp.rec[2 * at + 1] = make_int4(s.head, slot, 0, 0);
     }
+    ++turn;
+    if (shares && threadIdx.x == 0) kept[3 + (turn & 1)] = s.at + weight;      // two places: a walk, with its barriers, lies between a write and the next to its place
     walk(s, wt, x0, x1, slot);
     lanes.b0 = -64;            // read again, as these are
     sh.total = uniform(kept[0]), sh.used = uniform(kept[1]), hi = uniform(kept[2]);
     if (shares) {
-      done = uniform(s.at + weight);
+      s.at = done = uniform(kept[3 + (turn & 1)]);
       if (!(done < hi)) break;
       paged_next<ROWS>(p, lanes, s);
     }
