@@ -60,7 +60,6 @@ PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long ta
 // How a call is divided, from shapes alone: rows of an item (16, 32: one wavefront; 128: four) and work-groups.
 struct PagedPlan {
   int rows, W, items;      // items: as in PagedSplit
-  int shape() const { return rows == 16 ? 16 : 32; }
   size_t slots() const { return 2ull * W; }
   size_t rec_bytes() const { return (size_t)W * 2 * sizeof(int4); }
   size_t part_bytes(int D) const { return slots() * rows * D * 4; }

@@ -110,6 +110,10 @@ __device__ __forceinline__ PagedTotal paged_total(const PagedAttn& p, PagedLanes
   return PagedTotal{uniform(s.weight), uniform(s.most), uniform(s.items)};
 }
 
+// No 64-bit divisions below: each is some thirty instructions in series before a work-group's first load.  Where a quotient decides on a border, all that
+// matters is that everyone who asks gets the same, so an fp32 reciprocal serves; where it must be the floor, it is a guess that is put right.
+__device__ __forceinline__ double about(double x, double y) { return x * (double)__builtin_amdgcn_rcpf((float)y); }
+
 struct PagedItem {
   int b, head, t;          // b >= B: behind the last
   double at, index;        // weight and number of the items in front of it
@@ -138,9 +142,9 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, PagedLanes<R
   const PagedWeight w = lanes.of(p, s.b);
   const double one = NUMBERS ? (double)w.tiles : w.upto(w.tiles);      // of one head
   double r = x - (NUMBERS ? s.index : s.at);
-  int head = (int)fmin(floor(r / one), Hkv - 1.0), t = 0;
-  if (head > 0 && one * head > r) --head;
-  if (head + 1 < Hkv && one * (head + 1) <= r) ++head;
+  int head = (int)fmin(floor(about(r, one)), Hkv - 1.0), t = 0;
+  while (head > 0 && one * head > r) --head;
+  while (head + 1 < Hkv && one * (head + 1) <= r) ++head;
   r -= one * head;
   if (NUMBERS) {
     t = (int)fmin(r, w.tiles - 1.0);
@@ -168,18 +172,18 @@ __device__ __forceinline__ void paged_next(const PagedAttn& p, PagedLanes<ROWS>&
 
 // Shares: work-group `at` of `used` has the weights [bound(at), bound(at + 1)).
 struct PagedShares {
-  double total, used;
-  __device__ __forceinline__ double bound(int at) const { return uniform(floor(total * at / used)); }
+  double total, used, share;
+  __device__ __forceinline__ double bound(int at) const { return uniform(at >= used ? total : floor(share * at)); }
   __device__ __forceinline__ int holding(double x) const {      // the share that holds place x
-    int w = (int)floor(x * used / total);
+    int w = (int)fmin(floor(about(x, share)), used - 1);
     while (w > 0 && bound(w) > x) --w;
     while (w + 1 < used && bound(w + 1) <= x) ++w;
     return __builtin_amdgcn_readfirstlane(w);
   }
 };
 __device__ __forceinline__ PagedShares paged_shares(const PagedTotal& t, int W, int most_parts, double least) {      // least: weight that is worth a work-group
-  const double used = fmin(fmin((double)W, ceil(t.weight / least)), floor(t.weight * (most_parts - 2) / t.most));
-  return PagedShares{t.weight, uniform(fmax(used, 1.0))};
+  const double some = fmin(fmin((double)W, ceil(about(t.weight, least))), floor(about(t.weight * (most_parts - 2), t.most))), used = uniform(fmax(some, 1.0));
+  return PagedShares{t.weight, used, uniform(about(t.weight, used))};
 }
 // what a work-group walks of an item, in steps of KB keys: places x0 .. x1 of its weight
 struct PagedRange {
@@ -188,16 +192,31 @@ struct PagedRange {
 template <int KB>
 __device__ __forceinline__ PagedRange paged_range(double x0, double x1, double weight, int k_end) {
   const int steps = (k_end + KB - 1) / KB;
-  const int s0 = __builtin_amdgcn_readfirstlane((int)floor(x0 * steps / weight)), s1 = __builtin_amdgcn_readfirstlane((int)floor(x1 * steps / weight));
+  const double each = about((double)steps, weight);
+  const int s0 = __builtin_amdgcn_readfirstlane(min((int)floor(x0 * each), steps)), s1 = x1 >= weight ? steps : __builtin_amdgcn_readfirstlane(min((int)floor(x1 * each), steps));
   return PagedRange{s0 * KB, min(k_end, s1 * KB)};
 }
-// the keys that rows r0 .. r0 + n - 1 of a sequence see at all, and those that all of them see
+// Rows r0 .. of a sequence (r0 the same in all lanes): row r0 + i, i below 128, is token `token(i)`, head `head(i)` of the group.
+struct PagedRowsAt {
+  int tok, rem, G;
+  __device__ __forceinline__ PagedRowsAt(int r0, int G_) : G(G_) { tok = __builtin_amdgcn_readfirstlane(r0 / G), rem = r0 - tok * G; }
+  __device__ __forceinline__ void of(int i, int& token, int& head) const {
+    const int n = rem + i < (1 << 20) ? small_div(rem + i, G) : (rem + i) / G;      // small_div reaches 2^21
+    token = tok + n, head = rem + i - n * G;
+  }
+  __device__ __forceinline__ int token(int i) const {
+    int t, h;
+    of(i, t, h);
+    return t;
+  }
+};
+// the keys that rows i .. i + n - 1 behind `at` see at all, and those that all of them see; `rows` of the sequence's rows are behind `at`
 struct PagedSight {
   int most, least;
 };
-__device__ __forceinline__ PagedSight paged_sight(const PagedAttn& p, const PagedWeight& w, int r0, int n) {
+__device__ __forceinline__ PagedSight paged_sight(const PagedAttn& p, const PagedWeight& w, const PagedRowsAt& at, int i, int n, int rows) {
   if (!p.causal) return PagedSight{w.len, w.len};
-  const int rows = w.nq * p.G, last = (min(r0 + n, rows) - 1) / p.G, first = r0 / p.G;
+  const int first = at.token(i), last = at.token(max(min(i + n, rows) - 1, i));
   return PagedSight{min(max(w.len - w.nq + last + 1, 0), w.len), min(max(w.len - w.nq + first + 1, 0), w.len)};
 }
 __device__ __forceinline__ int paged_table_at(const PagedView& c, int b, int i) {      // by the scalar unit: b and i are the same in all lanes.  As it stands: not yet held inside the cache

@@ -165,7 +165,6 @@ struct PagedRows {
   static constexpr int CPR = RBY / 16, RPI = 1024 / RBY, IPG = 16 / RPI;
   static constexpr int NBUF = 2, TILE = KB * RBY, BUF = 2 * TILE, SCALES = NBUF * BUF, LDS = NBUF * BUF + (FP8 ? NBUF * 2 * KB * 4 : 0);
   static constexpr int LOADS = 2 * NG * IPG + (FP8 ? 2 : 0);      // vector-memory instructions of a step
-  static constexpr int LEAST = 4;                                 // steps that are worth a wavefront
 };
 
 // eight codes of two registers of the transposing reads, one of two columns each -> bf16
@@ -182,8 +181,9 @@ struct PagedWalk {
   const PagedSplit& sp;
   const int lane, w;
   uint32_t voff_k[C::IPG], voff_v[C::IPG];      // a lane's place in the rows of an instruction
-  int pg[C::NG];
+  int first_pg[C::NBUF - 1][C::NG], pg[C::NG];      // as the table has them
   int head, b, q0, nq, len, rows, r0, k_end, all_see, k0, k1;      // the stretch at hand
+  int first_tok, first_rem;      // row r0
   bool begins, ends;
 
   template <class Swz>
@@ -196,15 +196,16 @@ struct PagedWalk {
       voff_v[i] = (uint32_t)(row * p.c.v_st[1] * C::ES) + chunk * 16;
     }
   }
-  __device__ __forceinline__ void look_up(int kb) {
+  __device__ __forceinline__ void look_up(int (&to)[C::NG], int kb) const {
 #pragma unroll
-    for (int g = 0; g < C::NG; ++g) pg[g] = paged_table_at(p.c, b, (kb + 16 * g) >> p.c.page_log2);
+    for (int g = 0; g < C::NG; ++g) to[g] = paged_table_at(p.c, b, (kb + 16 * g) >> p.c.page_log2);
   }
   // the step at kb into buffer buf; behind the stretch: as many loads, of no rows
-  __device__ __forceinline__ void fetch(char* smem, int buf, int kb) {
+  __device__ __forceinline__ void fetch(char* smem, int buf, int kb, const int (&found)[C::NG]) {
+    int pg[C::NG];
     char* t = smem + buf * C::BUF;
 #pragma unroll
-    for (int g = 0; g < C::NG; ++g) pg[g] = min(max(pg[g], 0), p.c.num_pages - 1);      // here: in look_up it would wait for them
+    for (int g = 0; g < C::NG; ++g) pg[g] = min(max(found[g], 0), p.c.num_pages - 1);      // here: in look_up it would wait for them
     if constexpr (C::ES == 1) {
       const int j = max(min(kb + (lane & (C::KB - 1)), k1 - 1), kb), g = (j - kb) >> 4, place = j & ((1 << p.c.page_log2) - 1);
       int page = pg[0];
@@ -226,19 +227,26 @@ struct PagedWalk {
       }
     }
   }
+  // the pages of the first NBUF steps, asked for together
+  __device__ __forceinline__ void look_ahead() {
+#pragma unroll
+    for (int i = 0; i < C::NBUF - 1; ++i) look_up(first_pg[i], k0 + i * C::KB);
+    look_up(pg, k0 + (C::NBUF - 1) * C::KB);
+  }
   __device__ __forceinline__ void prologue(char* smem) {
 #pragma unroll
-    for (int i = 0; i < C::NBUF - 1; ++i) {
-      fetch(smem, i, k0 + i * C::KB);
-      look_up(k0 + (i + 1) * C::KB);
-    }
+    for (int i = 0; i < C::NBUF - 1; ++i) fetch(smem, i, k0 + i * C::KB, first_pg[i]);
   }
   // the loads of the step NBUF - 1 ahead go out, and this one's have landed
   __device__ __forceinline__ void turn(char* smem, int next, int kb) {
-    fetch(smem, next, kb + (C::NBUF - 1) * C::KB);
-    look_up(kb + C::NBUF * C::KB);
+    fetch(smem, next, kb + (C::NBUF - 1) * C::KB, pg);
+    look_up(pg, kb + C::NBUF * C::KB);
     FGRPO_WAIT_VMCNT((C::NBUF - 1) * C::LOADS);
     __builtin_amdgcn_sched_barrier(0);
+  }
+  __device__ __forceinline__ void row(int i, int& tok, int& hq) const {      // of the tile: its token in the sequence, its query head
+    const int n = first_rem + i < (1 << 20) ? small_div(first_rem + i, p.G) : (first_rem + i) / p.G;
+    tok = first_tok + n, hq = head * p.G + first_rem + i - n * p.G;
   }
   __device__ __forceinline__ int slot() const { return 2 * w + (begins ? 1 : 0); }
 
@@ -246,7 +254,7 @@ struct PagedWalk {
   __device__ __forceinline__ void run(Item&& item) {
     PagedLanes<ROWS> lanes;
     const PagedTotal total = paged_total<ROWS>(p, lanes);
-    const PagedShares sh = paged_shares(total, sp.W, sp.most_parts, (double)C::LEAST * C::KB * p.G);
+    const PagedShares sh = paged_shares(total, sp.W, sp.most_parts, (double)C::KB * p.G);
     const double hi = uniform(w < sh.used ? sh.bound(w + 1) : 0);
     double done = uniform(w < sh.used ? sh.bound(w) : 0);
     int4 rec = make_int4(0, 0, 0, 0);      // of the item that this wavefront begins and does not end
@@ -258,7 +266,9 @@ struct PagedWalk {
       const double weight = wt.of(s.t), x0 = done - s.at, x1 = fmin(hi - s.at, weight);
       b = s.b, head = s.head, q0 = wt.q0, nq = wt.nq, len = wt.len;
       rows = nq * p.G, r0 = s.t * ROWS;
-      const PagedSight sight = paged_sight(p, wt, r0, ROWS);
+      const PagedRowsAt at(r0, p.G);
+      first_tok = at.tok, first_rem = at.rem;
+      const PagedSight sight = paged_sight(p, wt, at, 0, ROWS, rows - r0);
       k_end = __builtin_amdgcn_readfirstlane(sight.most), all_see = __builtin_amdgcn_readfirstlane(sight.least);
       const PagedRange kr = paged_range<C::KB>(x0, x1, weight, k_end);
       k0 = kr.k0, k1 = kr.k1;
@@ -268,7 +278,7 @@ struct PagedWalk {
         const int i = min((int)s.index, sp.items - 1);
         sp.rec[2 * i] = ends ? make_int4(0, 0, 0, 0) : rec, sp.rec[2 * i + 1] = make_int4(head, 2 * w + 1, 0, 0);
       }
-      look_up(k0);
+      look_ahead();
       item();
       s.at = done = uniform(s.at + weight);
       if (done >= hi) break;
@@ -298,7 +308,8 @@ static __global__ __launch_bounds__(64) void paged_rows16_kernel(PagedAttn p, Pa
   const uint32_t tr_at = lds0 + C::TILE + tr_row * C::RBY + ((((r16 & 3) >> 1) ^ paged_swz16<C::RBY>(tr_row)) << 4) + 8 * (r16 & 1);
   const float c = p.scale * kLog2e;
   W.run([&]() {
-    const int row = min(W.r0 + r16, W.rows - 1), tok = row / p.G, hq = W.head * p.G + row % p.G;      // lanes behind the last row repeat it
+    int tok, hq;                 // lanes behind the last row repeat it
+    W.row(min(r16, W.rows - W.r0 - 1), tok, hq);
     const int seen = p.causal ? min(max(W.len - W.nq + tok + 1, 0), W.len) : W.len;
     bf16x8_t qf[KS];             // chunks as the K fragments have theirs (e4m3: 16 bytes are two steps' worth)
     const bf16_t* src = p.q + (long long)(W.q0 + tok) * p.q_t + (long long)hq * p.q_h;
@@ -443,7 +454,8 @@ static __global__ __launch_bounds__(64) void paged_rows_kernel(PagedAttn p, Page
   const PagedLane<C::RBY> L = paged_lane<C::RBY>(lane, lds0);
   const float c = p.scale * kLog2e;
   W.run([&]() {
-    const int row = min(W.r0 + (lane & 31), W.rows - 1), tok = row / p.G, hq = W.head * p.G + row % p.G;      // lanes behind the last row repeat it
+    int tok, hq;                 // lanes behind the last row repeat it
+    W.row(min(lane & 31, W.rows - W.r0 - 1), tok, hq);
     const int seen = p.causal ? min(max(W.len - W.nq + tok + 1, 0), W.len) : W.len;
     bf16x8_t qf[KS];             // chunks as the K fragments have theirs (e4m3: 16 bytes are two steps' worth)
     const bf16_t* src = p.q + (long long)(W.q0 + tok) * p.q_t + (long long)hq * p.q_h;

@@ -56,7 +56,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
   using C = PagedTiles<HD, FP8>;
   constexpr int KS = HD / 16, DB = HD / 32, G4 = KS / 2, ROWS = kPagedRows;
   __shared__ __attribute__((aligned(1024))) char smem[C::LDS];      // fragment addresses are formed by flipping bits below 1024
-  __shared__ double kept[5];
+  __shared__ double kept[6];
   const uint32_t lds0 = lds_addr(smem);
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int xcd = blockIdx.x & 7, n = sp.W >> 3, me = blockIdx.x >> 3, w = xcd * n + me;
@@ -83,11 +83,11 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     const bool whole = x0 <= 0 && x1 >= weight;
     const int q0 = wt.q0, nq = wt.nq, len = wt.len;
     const int rows = nq * p.G, r0 = s.t * ROWS, rw = r0 + 32 * wave;
-    const int k_end = __builtin_amdgcn_readfirstlane(paged_sight(p, wt, r0, ROWS).most);
+    const int k_end = __builtin_amdgcn_readfirstlane(paged_sight(p, wt, PagedRowsAt(r0, p.G), 0, ROWS, rows - r0).most);
     const PagedRange kr = paged_range<kAttnBK>(x0, x1, weight, k_end);
     const int k0 = kr.k0, k1 = kr.k1;
     const bool wave_on = rw < rows;
-    const PagedSight sight = paged_sight(p, wt, wave_on ? rw : r0, 32);
+    const PagedSight sight = paged_sight(p, wt, PagedRowsAt(r0, p.G), wave_on ? 32 * wave : 0, 32, rows - r0);
     const int w_most = wave_on ? __builtin_amdgcn_readfirstlane(sight.most) : 0, w_least = __builtin_amdgcn_readfirstlane(sight.least);
 
     int page = 0;
@@ -362,7 +362,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     rounds = items / n, left = items - rounds * n, parts = __builtin_amdgcn_readfirstlane(paged_last_parts(left, n));
     if (threadIdx.x == 0 && (me >= left || parts == 1)) sp.rec[2 * w] = none;      // record `me` of the XCD is its item `me` of the last round's
   }
-  if (threadIdx.x == 0) kept[0] = sh.total, kept[1] = sh.used, kept[2] = hi;      // what the walks must not carry in registers
+  if (threadIdx.x == 0) kept[0] = sh.total, kept[1] = sh.used, kept[2] = hi, kept[3] = sh.share;      // what the walks must not carry in registers
   __syncthreads();
   for (;;) {
     double x0 = 0, x1;
@@ -396,12 +396,12 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
       sp.rec[2 * at] = make_int4(rec, wt.q0, s.t * ROWS, wt.nq * p.G), sp.rec[2 * at + 1] = make_int4(s.head, slot, 0, 0);
     }
     ++turn;
-    if (shares && threadIdx.x == 0) kept[3 + (turn & 1)] = s.at + weight;      // two places: a walk, with its barriers, lies between a write and the next to its place
+    if (shares && threadIdx.x == 0) kept[4 + (turn & 1)] = s.at + weight;      // two places: a walk, with its barriers, lies between a write and the next to its place
     walk(s, wt, x0, x1, slot);
     lanes.b0 = -64;            // read again, as these are
-    sh.total = uniform(kept[0]), sh.used = uniform(kept[1]), hi = uniform(kept[2]);
+    sh.total = uniform(kept[0]), sh.used = uniform(kept[1]), hi = uniform(kept[2]), sh.share = uniform(kept[3]);
     if (shares) {
-      s.at = done = uniform(kept[3 + (turn & 1)]);
+      s.at = done = uniform(kept[4 + (turn & 1)]);
       if (!(done < hi)) break;
       paged_next<ROWS>(p, lanes, s);
     }
