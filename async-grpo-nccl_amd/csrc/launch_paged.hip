@@ -20,7 +20,8 @@ int check_cache(const char* who, const fgrpo_paged_cache* c, const int32_t* tabl
   if (c->num_blocks <= 0 || c->heads <= 0) return fail(FGRPO_ERR_BAD_ARG, "%s: num_blocks=%d heads=%d", who, c->num_blocks, c->heads);
   if (c->block_size < 16 || c->block_size > 65536 || (c->block_size & (c->block_size - 1)))
     return fail(FGRPO_ERR_UNSUPPORTED, "%s: block size %d (a power of two from 16 to 65536)", who, c->block_size);
-  if ((long long)width * c->block_size >= (1LL << 31)) return fail(FGRPO_ERR_UNSUPPORTED, "%s: a block table of %d blocks of %d reaches 2^31 tokens", who, width, c->block_size);
+  if ((long long)width * c->block_size > (1LL << 31) - 65536)      // places a few steps behind the last are formed in 32 bits
+    return fail(FGRPO_ERR_UNSUPPORTED, "%s: a block table of %d blocks of %d (at most 2^31 - 2^16 tokens)", who, width, c->block_size);
   if (c->head_dim != 128 && c->head_dim != 64) return fail(FGRPO_ERR_UNSUPPORTED, "%s: head dimension %d not supported (128 or 64)", who, c->head_dim);
   if (c->dtype != FGRPO_BF16 && c->dtype != FGRPO_F8E4M3) return fail(FGRPO_ERR_BAD_ARG, "%s: cache dtype=%d", who, c->dtype);
   const bool fp8 = c->dtype == FGRPO_F8E4M3;

@@ -223,7 +223,7 @@ __device__ __forceinline__ int paged_table_at(const PagedView& c, int b, int i) 
   const auto* row = (const __attribute__((address_space(4))) int*)(c.table + (long long)b * c.table_st);
   return row[min(i, c.width - 1)];
 }
-__device__ __forceinline__ float paged_lse(float m, float l) { return l > 0.f ? (m + __log2f(l)) * 0.6931471805599453f : -INFINITY; }
+__device__ __forceinline__ float paged_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + __log2f(l)) * 0.6931471805599453f; }      // l NaN: so is this
 
 // What a lane's accumulators hold.  SHAPE: rows of a block, 32 (v_mfma_f32_32x32x16_bf16) or 16 (16x16x32); the lane has row lane % SHAPE and, in unit u, four
 // columns: in blocks of 32 columns value 4 g + i of block db is unit 4 db + g, in blocks of 16 value i of block u is unit u.  PAIRS (the transposing reads

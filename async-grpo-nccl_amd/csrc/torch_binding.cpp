@@ -492,6 +492,7 @@ struct PagedBatch {
 PagedBatch paged_batch(const Tensor& k, const Tensor& v, const std::optional<Tensor>& k_scale, const std::optional<Tensor>& v_scale,
                        const Tensor& table, const Tensor& lens, const Tensor& cu) {
   PagedBatch b;
+  no_gradient(k, "a cache"), no_gradient(v, "a cache");
   TORCH_CHECK(k.dim() == 4 && k.sizes() == v.sizes(), "fgrpo: the cache is [num_blocks, block_size, heads, head_dim], got k ", k.sizes(), ", v ", v.sizes());
   TORCH_CHECK(k.scalar_type() == v.scalar_type() && (k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kFloat8_e4m3fn),
               "fgrpo: a cache is bf16 or float8_e4m3fn, got k ", k.scalar_type(), ", v ", v.scalar_type());
@@ -540,6 +541,7 @@ void paged_cache_write(const Tensor& k_cache, const Tensor& v_cache, const std::
 // an output the caller may bring
 Tensor output(const std::optional<Tensor>& given, at::IntArrayRef shape, at::ScalarType type, const Tensor& like, const char* name) {
   if (!given.has_value()) return at::empty(shape, like.options().dtype(type).requires_grad(false));
+  no_gradient(*given, name);
   require_one_gpu(like, *given);
   TORCH_CHECK(given->sizes() == shape && given->scalar_type() == type && given->is_contiguous() && aligned16(*given), "fgrpo: ", name, " must be ", type, " ", shape, ", contiguous and 16-byte aligned");
   return *given;
