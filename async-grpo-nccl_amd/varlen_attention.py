@@ -14,12 +14,16 @@ Mirrors, for this path, what the reference gets from flash-attn and from its loc
 * ``install_explicit_varlen_wrapper`` - the role of ``_install_explicit_fa2_varlen_wrapper``
   (``gpu_process_worker.py:110``): makes a model use the callable above; returns ``True`` when installed.
 
+Both functions also attend over a paged key/value cache (``fgrpo.ops.PagedCache``), without gradients: the first with
+``block_table``, the second with a ``PagedBatch``, which makes a Transformers model append to its caches and read
+them - for generation and for scoring continuations of what a cache already holds.
+
 There is no fallback: inputs the kernels do not cover (dropout, sliding windows, padding masks, head
 dimensions other than 128 and 64, CPU tensors) raise."""
 from __future__ import annotations
 
 import weakref
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -84,10 +88,15 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=Non
     the norm in bf16), and takes longer."""
     if dropout_p not in (0, 0.0):
         raise RuntimeError("fgrpo varlen attention: dropout is not supported (the reference passes 0.0)")
-    if tuple(window_size) != (-1, -1) or softcap not in (0, 0.0) or alibi_slopes is not None or block_table is not None:
-        raise RuntimeError("fgrpo varlen attention: window_size / softcap / alibi_slopes / block_table are not supported")
+    if tuple(window_size) != (-1, -1) or softcap not in (0, 0.0) or alibi_slopes is not None:
+        raise RuntimeError("fgrpo varlen attention: window_size / softcap / alibi_slopes are not supported")
     if return_attn_probs:
         raise RuntimeError("fgrpo varlen attention: attention probabilities are never materialised")
+    if block_table is not None:
+        if cu_seqlens_k.dim() != 1 or cu_seqlens_k.shape != cu_seqlens_q.shape:
+            raise RuntimeError("fgrpo varlen attention: with a block_table, cu_seqlens_k has an entry for each of cu_seqlens_q")
+        return ops.paged_attention(q, ops.PagedCache(k, v), block_table, (cu_seqlens_k[1:] - cu_seqlens_k[:-1]).to(torch.int32), cu_seqlens_q,
+                                   softmax_scale, bool(causal), _plain_length(max_seqlen_q))
     if cu_seqlens_q is not cu_seqlens_k:
         if cu_seqlens_q.shape != cu_seqlens_k.shape or not torch.equal(cu_seqlens_q, cu_seqlens_k):
             raise RuntimeError("fgrpo varlen attention: queries and keys must share their segments (self-attention)")
@@ -95,27 +104,68 @@ def flash_attn_varlen_func(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q=Non
     return ops.varlen_attention(q, k, v, cu_seqlens_q, softmax_scale, bool(causal), bounds, _plain_length(max_seqlen_q))
 
 
+class PagedBatch:
+    """What a Transformers model needs to run new tokens over paged caches: one ``ops.PagedCache`` a layer (``caches``, by the
+    attention modules' ``layer_idx``) and, shared by the layers, the blocks of each sequence (``block_table`` [sequences, blocks]
+    int32), its length with the new tokens (``seqused_k`` [sequences] int32) and where its new tokens lie in the packed row (``cu_seqlens``
+    [sequences + 1] int32).  ``max_len``: the most new tokens of a sequence, 0 where it is not known.  Passed to the model's
+    forward as ``paged_batch``, with ``input_ids`` / ``position_ids`` [1, T] and ``use_cache=False``: every attention layer writes its new
+    keys and values and attends over the cache."""
+
+    __slots__ = ("caches", "block_table", "seqused_k", "cu_seqlens", "max_len")
+
+    def __init__(self, caches: Sequence[ops.PagedCache], block_table: torch.Tensor, seqused_k: torch.Tensor, cu_seqlens: torch.Tensor,
+                 max_len: int = 0):
+        if not caches:
+            raise RuntimeError("fgrpo varlen attention: a paged batch has a cache for each layer")
+        self.caches, self.block_table, self.seqused_k, self.cu_seqlens = list(caches), block_table, seqused_k, cu_seqlens
+        self.max_len = _plain_length(max_len)
+
+    def reach(self) -> int:
+        """Tokens that the block table has places for."""
+        return self.block_table.shape[1] * self.caches[0].k.shape[1]
+
+
+def _paged_forward(module, query, key, value, scaling, is_causal, sliding_window, batch: PagedBatch):
+    B, Hq, L, D = query.shape
+    if B != 1:
+        raise RuntimeError("fgrpo varlen attention: a paged batch is one packed row ([1, T])")
+    if sliding_window is not None and sliding_window < batch.reach():
+        raise RuntimeError("fgrpo varlen attention: sliding-window attention is not supported")
+    layer = getattr(module, "layer_idx", None)
+    if layer is None or not 0 <= layer < len(batch.caches):
+        raise RuntimeError(f"fgrpo varlen attention: no cache for layer {layer} among {len(batch.caches)}")
+    q, k, v = (x[0].transpose(0, 1).to(torch.bfloat16) for x in (query, key, value))
+    cache = batch.caches[layer]
+    ops.paged_cache_write(cache, k, v, batch.block_table, batch.seqused_k, batch.cu_seqlens)
+    out = ops.paged_attention(q, cache, batch.block_table, batch.seqused_k, batch.cu_seqlens, scaling, is_causal, batch.max_len)
+    return out.view(1, L, Hq, D).to(query.dtype), None
+
+
 def varlen_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                              attention_mask: Optional[torch.Tensor] = None, dropout: float = 0.0,
                              scaling: Optional[float] = None, is_causal: Optional[bool] = None,
                              sliding_window: Optional[int] = None, position_ids: Optional[torch.Tensor] = None,
-                             **kwargs):
+                             paged_batch: Optional[PagedBatch] = None, **kwargs):
     """Attention callable in the Transformers attention-interface form: ``query`` [B, Hq, L, D], ``key`` /
     ``value`` [B, Hkv, L, D] -> ``(attn_output [B, L, Hq, D], None)``.  Segments come from ``position_ids``
     (every reset to 0 starts one, as in the reference wrapper); without ``position_ids`` every row is one
     segment.  A padding mask is not supported: packed batches carry none (the reference routes only
-    ``B == 1`` packed inputs to the varlen kernel)."""
+    ``B == 1`` packed inputs to the varlen kernel).  With ``paged_batch`` (``model(..., paged_batch=...)``) the keys and values
+    are appended to this layer's cache and the queries attend over it; positions then tell nothing about segments."""
     if dropout not in (0, 0.0):
         raise RuntimeError("fgrpo varlen attention: dropout is not supported")
-    B, Hq, L, D = query.shape
-    if sliding_window is not None and sliding_window < L:
-        raise RuntimeError("fgrpo varlen attention: sliding-window attention is not supported")
-    if key.shape[2] != L:
-        raise RuntimeError("fgrpo varlen attention: a key/value cache (keys longer than queries) is not supported")
-    if attention_mask is not None and attention_mask.dim() == 2 and not bool(attention_mask.all()):
-        raise RuntimeError("fgrpo varlen attention: padded batches are not supported; pack the samples instead")
     if is_causal is None:
         is_causal = bool(getattr(module, "is_causal", True))
+    B, Hq, L, D = query.shape
+    if paged_batch is None and sliding_window is not None and sliding_window < L:
+        raise RuntimeError("fgrpo varlen attention: sliding-window attention is not supported")
+    if key.shape[2] != L:
+        raise RuntimeError("fgrpo varlen attention: keys longer than queries come from paged caches (paged_batch) only")
+    if attention_mask is not None and attention_mask.dim() == 2 and not bool(attention_mask.all()):
+        raise RuntimeError("fgrpo varlen attention: padded batches are not supported; pack the samples instead")
+    if paged_batch is not None:
+        return _paged_forward(module, query, key, value, scaling, bool(is_causal), sliding_window, paged_batch)
     if position_ids is not None:
         cu, longest = prepare_from_position_ids(position_ids)
     else:

@@ -95,3 +95,55 @@ def test_torch_layer_refuses_before_it_takes_an_address():
         ops.PagedCache.empty(4, 16, 2, 128, torch.float16, "cpu")
     with pytest.raises(RuntimeError, match="unsupported dtype"):
         ops.verify_drafts(torch.zeros(2, 8, dtype=torch.float64), None, torch.zeros(2, dtype=torch.long), torch.zeros(2), cu)
+
+
+def test_callables_refuse(monkeypatch):
+    import varlen_attention as VA
+    from types import SimpleNamespace
+    from fgrpo import ops
+    kv = torch.zeros(4, 16, 2, 128, dtype=torch.bfloat16)
+    q, cu, table = torch.zeros(3, 4, 128, dtype=torch.bfloat16), torch.tensor([0, 1, 3], dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        VA.flash_attn_varlen_func(q, kv, kv, cu, cu, block_table=table)
+    with pytest.raises(RuntimeError, match="entry for each"):
+        VA.flash_attn_varlen_func(q, kv, kv, cu, cu[:2], block_table=table)
+    with pytest.raises(RuntimeError, match="gradient"):
+        VA.flash_attn_varlen_func(q, kv.clone().requires_grad_(True), kv, cu, cu, block_table=table)
+    for name, value in (("dropout_p", 0.1), ("window_size", (5, 0)), ("softcap", 1.0), ("return_attn_probs", True)):
+        with pytest.raises(RuntimeError, match="fgrpo varlen attention"):
+            VA.flash_attn_varlen_func(q, kv, kv, cu, cu, block_table=table, **{name: value})
+    with pytest.raises(RuntimeError, match="cache for each layer"):
+        VA.PagedBatch([], table, cu[1:], cu)
+    batch = VA.PagedBatch([ops.PagedCache(kv, kv)], table, cu[1:], cu)
+    assert batch.reach() == 64
+    x, y = torch.zeros(1, 4, 3, 128, dtype=torch.bfloat16), torch.zeros(1, 2, 3, 128, dtype=torch.bfloat16)
+    layer = SimpleNamespace(layer_idx=0, is_causal=True)
+    with pytest.raises(RuntimeError, match="GPU"):
+        VA.varlen_attention_forward(layer, x, y, y, paged_batch=batch)
+    with pytest.raises(RuntimeError, match="no cache for layer 1"):
+        VA.varlen_attention_forward(SimpleNamespace(layer_idx=1), x, y, y, paged_batch=batch)
+    with pytest.raises(RuntimeError, match="no cache for layer None"):
+        VA.varlen_attention_forward(SimpleNamespace(), x, y, y, paged_batch=batch)
+    with pytest.raises(RuntimeError, match="one packed row"):
+        VA.varlen_attention_forward(layer, x.expand(2, -1, -1, -1), y.expand(2, -1, -1, -1), y.expand(2, -1, -1, -1), paged_batch=batch)
+    with pytest.raises(RuntimeError, match="sliding"):
+        VA.varlen_attention_forward(layer, x, y, y, sliding_window=63, paged_batch=batch)
+    with pytest.raises(RuntimeError, match="paged caches"):
+        VA.varlen_attention_forward(layer, x, y[:, :, :2], y[:, :, :2], paged_batch=batch)
+
+
+def test_tables_that_reach_the_end_of_32_bits(lib):
+    c = C.byref(_cache(block_size=65536))
+    assert _attend(lib, c, width=32768, table_st=32768) == -2 and b"2^31" in lib.fgrpo_last_error()
+    assert _attend(lib, c, width=32767, table_st=32767, ws_bytes=8) == -3          # this far it goes
+
+
+def test_outputs_and_caches_that_want_gradients():
+    from fgrpo import ops
+    kv = torch.zeros(4, 16, 2, 128, dtype=torch.bfloat16)
+    table, lens, cu = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.paged_attention(q, ops.PagedCache(kv, kv.clone().requires_grad_(True)), table, lens, cu)
+    with pytest.raises(RuntimeError, match="gradient"):
+        ops.paged_cache_write(ops.PagedCache(kv.clone().requires_grad_(True), kv), q[:, :2], q[:, :2], table, lens, cu)
