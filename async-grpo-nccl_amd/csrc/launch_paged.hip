@@ -2,6 +2,8 @@
 // (kernels in paged_cache.h, paged_attn.h, draft_kernels.h).
 #include <string.h>
 
+#include <algorithm>
+
 #include "host_common.h"
 #include "draft_kernels.h"
 #include "paged_tiles.h"
@@ -70,7 +72,7 @@ PagedPlan plan_paged(const fgrpo_paged_cache* c, int width, int n_seq, int T, in
   const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq, rows = tokens * G;      // not known: the mean
   PagedPlan r{rows <= 16 ? 16 : rows <= 64 ? 32 : kPagedRows, 0, 0};
   const long long items = ((long long)T * G / r.rows + n_seq) * c->heads, steps = ((long long)width * c->block_size + 63) / 64 + 1;
-  long long W = (r.rows == kPagedRows ? 2LL : 4LL) * num_cus();
+  long long W = r.rows == kPagedRows ? std::min(2LL * num_cus(), 512LL) : 4LL * num_cus();      // 512: a lane of a wavefront for each of an XCD's eighth
   if (items < W && items * steps < W) W = items * steps;
   r.W = (int)round_up(W, 8);
   if (r.rows != kPagedRows && 8 * items <= r.W) r.items = (int)items;

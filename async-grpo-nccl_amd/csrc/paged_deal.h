@@ -149,11 +149,11 @@ __device__ __forceinline__ PagedItem paged_item(const PagedAttn& p, PagedLanes<R
   if (NUMBERS) {
     t = (int)fmin(r, w.tiles - 1.0);
   } else {
-    for (int low = 0, high = w.tiles - 1; low <= high;) {      // the last tile that begins at r or before
-      const int mid = (low + high) / 2;
-      if (w.upto(mid) <= r) t = mid, low = mid + 1;
-      else high = mid - 1;
-    }
+    // the last tile that begins at r or before: base n + slope n (n + 1) / 2 = r, solved in fp32 and put right
+    const float m = (float)w.base + 0.5f * (float)w.slope, x = (float)r;
+    t = (int)fminf(2.f * x * __builtin_amdgcn_rcpf(m + __builtin_amdgcn_sqrtf(m * m + 2.f * (float)w.slope * x)), (float)(w.tiles - 1));
+    while (t > 0 && w.upto(t) > r) --t;
+    while (t + 1 < w.tiles && w.upto(t + 1) <= r) ++t;
   }
   s.head = __builtin_amdgcn_readfirstlane(head), s.t = __builtin_amdgcn_readfirstlane(t);
   s.at = uniform(s.at + w.upto(w.tiles) * s.head + w.upto(s.t)), s.index = uniform(s.index + (double)w.tiles * s.head + s.t);
