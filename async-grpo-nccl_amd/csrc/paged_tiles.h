@@ -43,6 +43,14 @@ __device__ __forceinline__ AttnTr paged_rd_tr(uint32_t a) {      // attn_rd_tr_a
   return f;
 }
 
+template <int OFF>
+__device__ __forceinline__ uint32_t paged_read_u32(uint32_t a) {
+  uint32_t x;
+  asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(x) : "v"(a), "i"(OFF));
+  return x;
+}
+__device__ __forceinline__ void paged_settle_u32(uint32_t& x) { asm volatile("" : "+v"(x)); }
+
 // Parts of the last, incomplete round of `left` items (fewer than n) on `n` work-groups: the shortest of rounds / parts, a cut costing about a 20th of an item.
 __device__ __forceinline__ int paged_last_parts(int left, int n) {
   int best = 1;
@@ -95,6 +103,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     const AttnLane<HD> L = attn_lane<HD>(lane);
     row_at = L.rowc[0] + lds0, tr_at[0] = L.tr[0][0] + lds0, tr_at[1] = L.tr[0][1] + lds0;
   }
+  const uint32_t sc_at = lds0 + (8 * ((lane & 15) >> 2) + (lane & 3) + 4 * h) * 4;
   const float c = p.scale * kLog2e;
   // where this wavefront's lanes read: row lane / CPR of 16 and every RPI-th behind it, and of instruction i chunk `ch`, but for the bits of
   // the swizzle that i decides; and, codes, where they write
@@ -182,7 +191,7 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
     for (int db = 0; db < DB; ++db)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[db][r] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;      // the maximum in powers of two
+    float m_run = -INFINITY, m_at = 0.f, l_run = 0.f;      // the maximum in powers of two, as the sums have it; the same, but 0 for none
     bool started = false;
     if constexpr (FP8) {
       if (k0 < k1) put_codes(I0{});
@@ -234,20 +243,21 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
             s2[g / 2] = attn_mfma(kf[g % 2][i], __builtin_bit_cast(u32x4_t, qf[G4 * (g % 2) + i]), s2[g / 2]);
           }
         };
-        u32x4_t sk[4];              // scales of the 32 keys of a half, of K and then of V
-        auto req_scales = [&](auto mbc, auto which) {
-          constexpr int mb = decltype(mbc)::value;
+        // Scales of the 32 keys of a half, of K and of V: the lane has that of score lane % 16, and a row of 16 lanes hands them to each other as operands
+        uint32_t sc[4];
+        if constexpr (FP8)
           static_for<4>([&](auto ic) {
             constexpr int i = decltype(ic)::value;
-            sk[i] = lds_read_u128_asm<cur * 2 * kAttnBK * 4 + decltype(which)::value * kAttnBK * 4 + mb * 128 + 32 * i>(lds0 + 16 * h);
+            sc[i] = paged_read_u32<cur * 2 * kAttnBK * 4 + i * 128>(sc_at);
           });
-        };
-        auto scale_half = [&](auto mbc) {
-          constexpr int mb = decltype(mbc)::value;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) attn_settle(sk[i]);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s2[mb][r] *= __uint_as_float(sk[r >> 2][r & 3]);
+        auto scale_half = [&](auto mbc, auto which) {
+          constexpr int mb = decltype(mbc)::value, i = 2 * decltype(which)::value + mb;
+          static_for<16>([&](auto rc) {
+            constexpr int r = decltype(rc)::value;
+            float x = s2[mb][r] * __uint_as_float(__builtin_amdgcn_mov_dpp(sc[i], 0x150 + r, 0xf, 0xf, true));      // row_newbcast
+            asm volatile("" : "+v"(x));      // here, not in the blocks that use it: the broadcast is an operand only within one
+            s2[mb][r] = x;
+          });
         };
         __builtin_amdgcn_s_setprio(1);      // the other work-group's wavefront on this SIMD does its softmax beside the products
         req_k(I0{});
@@ -267,22 +277,15 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
         __builtin_amdgcn_sched_barrier(0);
         mma_k(I2{});
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (FP8) req_scales(I0{}, I0{});
-        wait_lgkm<2 * DB + (FP8 ? 4 : 0)>();
+        wait_lgkm<2 * DB>();
         __builtin_amdgcn_sched_barrier(0);
         mma_k(I3{});
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (FP8) {
-          wait_lgkm<0>();
-          __builtin_amdgcn_sched_barrier(0);
-          scale_half(I0{});
-          __builtin_amdgcn_sched_barrier(0);
-          req_scales(I1{}, I0{});
-          wait_lgkm<0>();
-          __builtin_amdgcn_sched_barrier(0);
-          scale_half(I1{});
-          __builtin_amdgcn_sched_barrier(0);
-          req_scales(I0{}, I1{});
+#pragma unroll
+          for (int i = 0; i < 4; ++i) paged_settle_u32(sc[i]);      // these landed first
+          scale_half(I0{}, I0{});
+          scale_half(I1{}, I0{});
         }
         __builtin_amdgcn_s_setprio(0);
         float mx = -INFINITY;
@@ -303,36 +306,36 @@ static __global__ __launch_bounds__(256, 2) void paged_tiles_kernel(PagedAttn p,
           attn_halves(mx, mlo, mhi);
           mx = fmaxf(mlo, mhi);
         }
-        const float m_new = fmaxf(m_run, mx * c), m_use = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m_run - m_use);
+        // The sums' power of two follows the maximum once it is 2^8 behind for some row: numerators stay below 2^8, and most steps have nothing to rescale
+        const float m_new = fmaxf(m_run, mx * c);
+        if (__any(m_new - m_run > 8.f)) {
+          const float m_use = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m_run - m_use);
+          m_run = m_new, m_at = m_use, l_run *= alpha;
+          if (started) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+          }
+        }
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float e = fast_exp2(__builtin_fmaf(s2[mb][r], c, -m_use));
+            const float e = fast_exp2(__builtin_fmaf(s2[mb][r], c, -m_at));
             s2[mb][r] = e;
             sum[mb] += e;
           }
-        l_run = l_run * alpha + (sum[0] + sum[1]);
-        m_run = m_new;
-        if (started && __any(alpha != 1.f)) {
-#pragma unroll
-          for (int db = 0; db < DB; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
-        }
+        l_run += sum[0] + sum[1];
         if constexpr (FP8) {
-          wait_lgkm<0>();
-          __builtin_amdgcn_sched_barrier(0);
-          scale_half(I0{});
-          __builtin_amdgcn_sched_barrier(0);
-          req_scales(I1{}, I1{});      // lands with the next group's columns
+          scale_half(I0{}, I1{});
+          scale_half(I1{}, I1{});
         }
         __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_setprio(1);
         static_for<4>([&](auto qc) {
           constexpr int q = decltype(qc)::value, mb = q / 2, half = q % 2;
-          if constexpr (FP8 && q == 2) scale_half(I1{});
           if constexpr (q < 3) req_v(std::integral_constant<int, q + 1>{});
           wait_lgkm<(q < 3 ? 2 * DB : 0)>();
           __builtin_amdgcn_sched_barrier(0);
