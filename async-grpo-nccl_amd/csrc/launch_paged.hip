@@ -61,6 +61,11 @@ PagedView view_of(const fgrpo_paged_cache* c, const int32_t* table, long long ta
   } while (0)
 
 // How a call is divided, from shapes alone: rows of an item (16, 32: one wavefront; 128: four) and work-groups.
+// Up to 16 rows a sequence and K/V head take blocks of 16 (64 sequences of 1000 .. 4000 keys, 12 / 2 heads, bf16: 38 us, blocks of 32 42; e4m3 32.5, 36).
+// Every block reads its keys, from L2 but for the first, so with many blocks tiles of 128 win, and with few their larger parts and merges cost more than that: us,
+// 32 / 128, bf16, D = 128, by blocks x keys that the table has room for: 128 K 25 / 46 (4 sequences to 16000) and 21 / 28 (16 to 4000),
+// 384 K 27 / 37, 512 K 38 / 62, 50 / 77, 40 / 39, 39 / 36 and 43 / 39 (from 4 sequences to 64), 768 K 47 / 38, 1 M 60 / 45, 57 / 42, 85 / 84, 2 M 100 / 51, 220 / 146;
+// D = 64: 256 K 21 / 30, 512 K 26 / 24, 640 K 25 / 27, 1 M 36 / 29; e4m3 alike.  So: 512 K.  One block a sequence is never far behind (75 / 72, 43 / 39; e4m3 89 / 111).
 struct PagedPlan {
   int rows, W, items;      // items: as in PagedSplit
   size_t slots() const { return 2ull * W; }
@@ -70,11 +75,13 @@ struct PagedPlan {
 };
 PagedPlan plan_paged(const fgrpo_paged_cache* c, int width, int n_seq, int T, int G, int max_len) {
   const long long tokens = max_len > 0 ? (max_len < T ? max_len : T) : ((long long)T + n_seq - 1) / n_seq, rows = tokens * G;      // not known: the mean
-  PagedPlan r{rows <= 16 ? 16 : rows <= 64 ? 32 : kPagedRows, 0, 0};
+  const double blocks = ((double)T * G + 31.0 * n_seq) / 32 * c->heads, keys = (double)width * c->block_size;
+  PagedPlan r{rows <= 16 ? 16 : rows <= 32 || blocks * keys <= 512 * 1024 ? 32 : kPagedRows, 0, 0};
   const long long items = ((long long)T * G / r.rows + n_seq) * c->heads, steps = ((long long)width * c->block_size + 63) / 64 + 1;
   long long W = r.rows == kPagedRows ? std::min(2LL * num_cus(), 512LL) : 4LL * num_cus();      // 512: a lane of a wavefront for each of an XCD's eighth
   if (items < W && items * steps < W) W = items * steps;
   r.W = (int)round_up(W, 8);
+  // few items, many parts: merged an item's unit a work-group (one sequence of 100000 keys 54 us, else 94; 16 of 1000 .. 4000 17.2, 25.7; 32 of them 23.7, 27.8)
   if (r.rows != kPagedRows && 8 * items <= r.W) r.items = (int)items;
   return r;
 }
@@ -204,7 +211,8 @@ int fgrpo_verify_drafts(const void* target, long long target_stride, const void*
   VerifyParams p{target, draft, (const long long*)ids, u, cu_seqlens, target_stride, draft_stride, n_seq, T, V, draft_rows, verify_chunks(V), accepted, (long long*)tokens,
                  (double2*)ws, (int*)((char*)ws + verify_sums_bytes(n_seq, V))};
   const bool f32 = dtype == FGRPO_F32;
-  const long long es = f32 ? 4 : 2;      // rows that begin at multiples of 16 bytes are read 16 bytes at a time: half the time of a vocabulary of 32000, where loads are in short supply
+  // rows that begin at multiples of 16 bytes are read 16 bytes at a time (64 sequences, 151936 tokens, bf16: 19.0 us, else 31.7; fp32 23.4, 34.5; 32000 tokens 12.6, 17.4)
+  const long long es = f32 ? 4 : 2;
   const bool whole = aligned16(target) && target_stride * es % 16 == 0 && (!draft || (aligned16(draft) && draft_stride * es % 16 == 0));
   hipStream_t st = (hipStream_t)stream;
   if (f32) return whole ? launch_verify<true, true>(p, st) : launch_verify<true, false>(p, st);

@@ -1200,8 +1200,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, block_table: torch.Tenso
     ``causal`` those with ``j <= seqused_k[b] - n + i``.  Query head ``h`` reads K/V head ``h // (Hq // heads)``.  One token a sequence,
     drafts, and pieces of prompts may share a call.  Returns [T, Hq, head_dim] bf16, with ``return_lse`` also the log of
     the softmax denominators, fp32 [Hq, T].  A row that sees nothing gives 0 and -inf; rows behind the last sequence are left as
-    they are in ``out``, and hold anything without it.  ``max_len``: the most new tokens of a sequence, 0 where it is not known:
-    the kernel is chosen by it, results do not depend on it but for the order of fp32 sums.  Values that a query does
+    they are in ``out``, and hold anything without it.  ``max_len``: the most new tokens of a sequence, 0 where it is not known.  The kernel is
+    chosen by it and by how many tokens ``block_table`` is wide enough for (hand over the columns that the longest sequence needs); results
+    do not depend on either but for the order of fp32 sums.  Values that a query does
     not see are not read, but for V of keys that other queries of its sequence in the same call see: those must be finite.  No
     gradient, no host wait."""
     got = _lib.native().paged_attention(q, cache.k, cache.v, cache.k_scale, cache.v_scale, block_table, seqused_k, cu_seqlens,

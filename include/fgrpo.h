@@ -397,7 +397,7 @@ int fgrpo_varlen_attn_bwd_len(const void* dout, const void* q, const void* k, co
  * The three calls share their description of a batch: block_table [n_seq][width] int32 (rows table_stride entries apart): the
  * block of a sequence's tokens i*block_size ..; seqused_k [n_seq] int32: a sequence's length, new tokens included;
  * cu_seqlens [n_seq+1] int32: its rows in the packed arrays.  All on the device, read by the kernels, held inside their arrays
- * there: cu_seqlens in [0, T], lengths in [0, width*block_size], blocks in [0, num_blocks).
+ * there: cu_seqlens in [0, T], lengths in [0, width*block_size], blocks in [0, num_blocks).  width*block_size is at most 2^31 - 2^16.
  * write: row cu[b]+i of k / v [T][heads][head_dim] bf16 (strides in elements, multiples of 8) goes to position
  * seqused_k[b] - (cu[b+1]-cu[b]) + i of sequence b; rows whose position is negative, and rows behind cu[n_seq], go nowhere.
  * e4m3: scale = max(max |finite x|, 1e-30) / 448 over a row's head_dim values, code = x * (448 / that max) rounded to nearest even;
@@ -423,8 +423,8 @@ int fgrpo_paged_cache_read(const fgrpo_paged_cache* cache, const int32_t* block_
  * ones of sequence b and sees its keys j < seqused_k[b], with causal != 0 those with j <= seqused_k[b] - q_b + i.  Query head h reads K/V
  * head h / (Hq/heads).  out [T][Hq][head_dim] bf16 contiguous; lse [Hq][T] fp32 or NULL (natural log of the softmax
  * denominator).  A row that sees nothing: out 0, lse -inf.  Rows behind cu[n_seq] are left as they are.  No gradient.
- * max_len: the most rows of a sequence, 0 where it is not known: the kernel and its workspace are chosen by it, results do not depend on it
- * but for the order of fp32 sums.  ws: 16-byte aligned, fgrpo_paged_attn_workspace bytes for the same arguments (0: may be NULL); nothing in it has
+ * max_len: the most rows of a sequence, 0 where it is not known.  The kernel and its workspace are chosen by it and by `width` (hand over the
+ * columns that the longest sequence needs); results do not depend on either but for the order of fp32 sums.  ws: 16-byte aligned, fgrpo_paged_attn_workspace bytes for the same arguments (0: may be NULL); nothing in it has
  * to start at zero, and calls that overlap need one each. */
 size_t fgrpo_paged_attn_workspace(const fgrpo_paged_cache* cache, int width, int n_seq, int T, int Hq, int max_len);
 int fgrpo_paged_attn_fwd(const void* q, long long q_stride_t, long long q_stride_h, const fgrpo_paged_cache* cache,

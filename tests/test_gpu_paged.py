@@ -29,11 +29,12 @@ def _table(lens, block, width, pages, rng):
     return table
 
 
-def _batch(qs, ks, Hq, Hkv, D, block, fp8, seed, tail=3, spare=2, nan=True):
-    """A batch on the CPU: packed queries with ``tail`` rows behind the last sequence, and a cache whose unused places are NaN."""
+def _batch(qs, ks, Hq, Hkv, D, block, fp8, seed, tail=3, spare=2, nan=True, reach=0):
+    """A batch on the CPU: packed queries with ``tail`` rows behind the last sequence, and a cache whose unused places are NaN.
+    ``reach``: tokens that the table has room for at least.  What a call is divided by goes by that and by ``max_len``."""
     g, rng = torch.Generator().manual_seed(seed), random.Random(seed)
     need = [(n + block - 1) // block for n in ks]
-    pages, width = sum(need) + spare, max(need + [0]) + 1
+    pages, width = sum(need) + spare, max(max(need + [0]) + 1, reach // block)
     table = _table(ks, block, width, pages, rng)
     cu = torch.tensor([0] + torch.tensor(qs).cumsum(0).tolist(), dtype=torch.int32)
     lens = torch.tensor(ks, dtype=torch.int32)
@@ -98,9 +99,9 @@ def test_attention_over_the_cache(dev, shape, Hq, Hkv, D, fp8):
     qs, ks = SHAPES[shape]
     block = (16, 64, 32, 256)[shape % 4]
     for causal in (True, False):
-        s = _batch(qs, ks, Hq, Hkv, D, block, fp8, seed=shape)
-        out = torch.full((s["T"], Hq, D), 7.0, dtype=torch.bfloat16, device=dev)
-        for hint in (max(qs), 0):
+        for hint, reach in ((max(qs), 0), (0, 0), (64, 1 << 20)):
+            s = _batch(qs, ks, Hq, Hkv, D, block, fp8, seed=shape, reach=reach)
+            out = torch.full((s["T"], Hq, D), 7.0, dtype=torch.bfloat16, device=dev)
             got, lse = ops.paged_attention(s["q"].to(dev), _cache(s, dev), s["table"].to(dev), s["lens"].to(dev), s["cu"].to(dev), causal=causal,
                                            max_len=hint, return_lse=True, out=out)
             assert got.data_ptr() == out.data_ptr()

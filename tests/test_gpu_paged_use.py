@@ -22,7 +22,7 @@ def _dev(s, dev):
 def test_layouts(dev, qs, ks, fp8):
     """Heads in front of tokens in a block, K and V side by side in one allocation, queries inside a wider row, a wider 64-bit table."""
     Hq, Hkv, D, block = 6, 3, 128, 32
-    s = _batch(qs, ks, Hq, Hkv, D, block, fp8, seed=11)
+    s = _batch(qs, ks, Hq, Hkv, D, block, fp8, seed=11, reach=(1 << 20) * (max(qs) > 64))
     q, table, lens, cu = _dev(s, dev)
     want, wl = ops.paged_attention(q, _cache(s, dev), table, lens, cu, return_lse=True, max_len=max(qs))
     _check(s, want, wl)
@@ -69,7 +69,7 @@ def test_many_sequences(dev, n, ks, fp8):
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("n,hint", [(1, 1), (1, 500), (5, 1), (5, 0), (150, 1), (150, 5), (150, 2 ** 30)])
 def test_one_long_sequence_in_many_parts_and_wrong_hints(dev, n, hint, fp8):
-    s = _batch([n], [30001], 12, 2, 128, 64, fp8, seed=n, nan=False)
+    s = _batch([n], [30001], 12, 2, 128, 64, fp8, seed=n, nan=False, reach=(1 << 20) * (hint > 8))
     q, table, ln, cu = _dev(s, dev)
     out, lse = ops.paged_attention(q, _cache(s, dev), table, ln, cu, return_lse=True, max_len=hint)
     again, _ = ops.paged_attention(q, _cache(s, dev), table, ln, cu, return_lse=True, max_len=hint)
@@ -85,8 +85,10 @@ def test_shared_blocks(dev, fp8):
     s = _batch([1, 3, 1], [prompt + n for n in own], Hq, Hkv, D, block, fp8, seed=4, nan=False)
     s["table"][1:, :prompt // block] = s["table"][0, :prompt // block]
     q, table, ln, cu = _dev(s, dev)
-    for hint in (3, 100):
-        out, lse = ops.paged_attention(q, _cache(s, dev), table, ln, cu, return_lse=True, max_len=hint)
+    for hint, reach in ((3, 0), (100, 1 << 20)):
+        wide = torch.full((3, max(table.shape[1], reach // block)), -1, dtype=torch.int32, device=dev)
+        wide[:, :table.shape[1]] = table
+        out, lse = ops.paged_attention(q, _cache(s, dev), wide, ln, cu, return_lse=True, max_len=hint)
         _check(s, out, lse)
 
 
@@ -96,7 +98,7 @@ def test_blocks_behind_32_bits(dev, Hq, n, fp8):
     """A cache whose last blocks begin behind 2^32 elements."""
     Hkv, D, block, pages = 8, 128, 64, 66000
     assert (pages - 10) * block * Hkv * D > 2 ** 32
-    s = _batch([n, n], [130, 300], Hq, Hkv, D, block, fp8, seed=9, spare=0, nan=False)
+    s = _batch([n, n], [130, 300], Hq, Hkv, D, block, fp8, seed=9, spare=0, nan=False, reach=(1 << 20) * (n > 32))
     need = s["k"][0].shape[0]
     at = [pages - 1 - i if i % 2 else i for i in range(need)]                  # far and near in turn
     big = [torch.empty(pages, block, Hkv, D, dtype=FP8 if fp8 else torch.bfloat16, device=dev) for _ in range(2)]
@@ -127,7 +129,7 @@ def test_blocks_behind_32_bits(dev, Hq, n, fp8):
 def test_masked_keys_may_hold_anything_and_seen_ones_count(dev, n, fp8):
     """A NaN in a key makes NaN of the rows that see it and of no others."""
     Hq, Hkv, D, block, L = 4, 2, 128, 16, 100
-    s = _batch([n], [L], Hq, Hkv, D, block, fp8, seed=2, nan=False)
+    s = _batch([n], [L], Hq, Hkv, D, block, fp8, seed=2, nan=False, reach=(1 << 20) * (n > 32))
     j = L - 1 - n // 2                           # seen by the last n // 2 + 1 rows
     page, at = PO.place(s["table"], 0, j, block)
     clean, _, _ = PO.attention(s["q"], PO.held(*s["k"]), PO.held(*s["v"]), s["table"], s["lens"], s["cu"], block)
@@ -150,7 +152,7 @@ def test_masked_keys_may_hold_anything_and_seen_ones_count(dev, n, fp8):
 def test_values_out_of_range_stay_inside(dev, hint, fp8):
     """Lengths, cu_seqlens and blocks from device memory that fit nothing are held inside their arrays; the sequences that are right are right."""
     Hq, Hkv, D, block = 4, 2, 64, 16
-    s = _batch([2, 4, 3, 6], [30, 40, 50, 60], Hq, Hkv, D, block, fp8, seed=8, nan=False)
+    s = _batch([2, 4, 3, 6], [30, 40, 50, 60], Hq, Hkv, D, block, fp8, seed=8, nan=False, reach=(1 << 20) * (hint > 8))
     q, table, ln, cu = _dev(s, dev)
     want = ops.paged_attention(q, _cache(s, dev), table, ln, cu, max_len=hint)
     reach = table.shape[1] * block
@@ -163,7 +165,7 @@ def test_values_out_of_range_stay_inside(dev, hint, fp8):
         torch.cuda.synchronize()
         return out
     bad = table.clone()
-    bad[1] = torch.tensor([2 ** 31 - 1, -2 ** 31, 10 ** 6, -1, 5][:table.shape[1]], dtype=torch.int32)
+    bad[1, :5] = torch.tensor([2 ** 31 - 1, -2 ** 31, 10 ** 6, -1, 5], dtype=torch.int32)
     got = run(bad, ln, cu)
     assert torch.equal(got[:2], want[:2]) and torch.equal(got[6:15], want[6:15])
     long = ln.clone()
@@ -384,7 +386,7 @@ def test_captured_step_follows_new_lengths(dev, fp8):
 
 
 def test_two_streams_at_once(dev):
-    cases = [_batch([1] * 6, [500, 3, 70, 900, 33, 64], 8, 2, 128, 16, False, seed=21), _batch([300], [1200], 8, 2, 128, 16, True, seed=22)]
+    cases = [_batch([1] * 6, [500, 3, 70, 900, 33, 64], 8, 2, 128, 16, False, seed=21), _batch([300], [1200], 8, 2, 128, 16, True, seed=22, reach=1 << 20)]
     ins = [(*_dev(s, dev), _cache(s, dev)) for s in cases]
     want = [ops.paged_attention(q, c, t, ln, cu, max_len=64) for q, t, ln, cu, c in ins]
     streams = [torch.cuda.Stream() for _ in ins]
