@@ -81,8 +81,9 @@ PagedPlan plan_paged(const fgrpo_paged_cache* c, int width, int n_seq, int T, in
   long long W = r.rows == kPagedRows ? std::min(2LL * num_cus(), 512LL) : 4LL * num_cus();      // 512: a lane of a wavefront for each of an XCD's eighth
   if (items < W && items * steps < W) W = items * steps;
   r.W = (int)round_up(W, 8);
-  // few items, many parts: merged an item's unit a work-group (one sequence of 100000 keys 54 us, else 94; 16 of 1000 .. 4000 17.2, 25.7; 32 of them 23.7, 27.8)
-  if (r.rows != kPagedRows && 8 * items <= r.W) r.items = (int)items;
+  // Few items, many parts: merged an item's unit a work-group (one sequence of 100000 keys 54 us, else 94; 16 of 1000 .. 4000 17.2, 25.7; 48 of 128 .. 8000, 12 / 2
+  // heads, 43 and 46).  At half as many work-groups an item it is behind: 128 sequences of 1000 .. 4000 with four drafts 78 us, else 73.
+  if (r.rows != kPagedRows && 4 * items <= r.W) r.items = (int)items;
   return r;
 }
 

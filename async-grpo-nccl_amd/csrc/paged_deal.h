@@ -10,7 +10,6 @@
 
 namespace fgrpo {
 
-
 struct PagedSplit {
   int W;                 // work-groups of the launch, a multiple of 8
   int items;             // > 0: no more items than this, few enough for the merge to have work-groups for every unit of each: records go by item, not by work-group
@@ -309,6 +308,7 @@ static __global__ __launch_bounds__(256) void paged_merge_items_kernel(PagedAttn
   if (p.lse && unit == 0 && lane < SHAPE) p.lse[(long long)hq * p.c.T + tok] = paged_lse(sum.m, sum.l);
 }
 
+// (Both are a launch of 3 to 5 us; 500 parts of 128 rows, 64 KiB each, take 9.)
 // Adds up the parts of the item of record blockIdx.x in the order of the keys: work-group y takes block y of SHAPE rows, wavefront w the units w, w + 4 ..
 // of their columns.  RB: blocks of a tile.
 template <int HD, bool PAIRS, int SHAPE, int RB>

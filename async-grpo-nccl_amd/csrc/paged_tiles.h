@@ -2,19 +2,24 @@
 // vector arithmetic beside them.  (What is computed: paged_attn.h; how it is dealt out: paged_deal.h.)
 //
 // A work-group of four wavefronts has 128 rows of a sequence and K/V head, 32 a wavefront, and walks their keys 64 at a time through two
-// LDS buffers, with one barrier a step and the fragment schedule of varlen_attn_fwd2_kernel (attn_kernels.h): two
-// work-groups a CU, so that one wavefront's softmax runs beside another's matrix instructions.  Wavefront w fetches keys 16 w .. of
+// LDS buffers, with one barrier a step and the fragment schedule of varlen_attn_fwd2_kernel (attn_kernels.h), two work-groups a CU.  Wavefront w fetches keys 16 w .. of
 // a step, which lie in one page: one look-up by the scalar unit, a step ahead.
 // bf16 travels global -> LDS directly.  e4m3 is converted once for the four wavefronts: codes wait in registers for a step (16 of them), and
-// are written to LDS as bf16, which holds them exactly; the scales of a step's keys lie beside the tiles in LDS.
+// are written to LDS as bf16, which holds them exactly; the scales of a step's keys lie beside the tiles in LDS, a lane reads one of them, and the multiplications take
+// them out of other lanes (each lane reading all of its own: 1 % more).
 //
 // Dealing out: a launch of W work-groups, all resident.  Where the heaviest item is more than two mean shares, or there are fewer items than
-// work-groups, shares of the weights, cut inside items (a cut costs 64 KiB of sums written and read per part).  Else whole items, W / 8 a round for
-// the W / 8 work-groups of an XCD, alternately from either end (under the causal mask weights ascend); what is left for the last
-// round is cut into as many parts as make it shortest.  Work-groups me and me + W / 16 of an XCD share a CU: where there is one round, the heaviest
-// items go beside the lightest (12 / 2 heads, 8 sequences of 682 tokens: 37.2 -> 31.8 us; 256 .. 1024 tokens over 2000 .. 3000 keys: 110 -> 105 us, with what follows).
-// The older of two wavefronts on a SIMD wins whatever both could issue, so both drift into the same phase; with the priority raised for the
-// products, one's softmax runs beside the other's products (4096 tokens over 32768 keys, 40 / 8 heads: 2.61 -> 2.48 ms, 1.04 PFLOP/s; e4m3 3.09 -> 2.93 ms).
+// work-groups, shares of the weights, cut inside items (a cut costs 64 KiB of sums written and read per part: 8 sequences of 682 tokens from the start 63 us in
+// shares, 32 whole).  Else whole items, W / 8 a round for the W / 8 work-groups of an XCD, alternately from either end (under the causal mask weights
+// ascend); what is left for the last round is cut into as many parts as make it shortest.  Work-groups me and me + W / 16 of an XCD share a CU: where there
+// is one round, the heaviest items go beside the lightest (those 8 sequences 37 us without, 256 .. 1024 tokens over 2000 .. 3000 keys 110 and 105).
+//
+// What a step costs is its instructions: 1024 cycles of matrix instructions a wavefront (32 rows, 64 keys, head dimension 128) and about as many of vector ones, nearly one after the
+// other though two wavefronts share a SIMD (bf16 2030 cycles a wavefront step, e4m3 2700; matrix pipes 0.5 busy).  The older of the two wins whatever both could issue,
+// so both drift into the same phase; with the priority raised for the products, one's softmax runs beside the other's products (-4..-5 %), and
+// sums that are rescaled only when the maximum has grown by 2^8 save the rest (-4..-8 %).  Memory is not what a step waits for: touching its
+// lines two to four steps early costs 7..18 %.  40 / 8 heads, 4096 tokens over 32768 keys: bf16 2.36 ms (1.09 PFLOP/s), e4m3 2.80 ms (0.92); 8192 tokens
+// from the start 0.67 ms; 14 / 2 heads of 64, 4096 over 32768, 0.57 ms.
 #pragma once
 #include "paged_rows.h"
 
