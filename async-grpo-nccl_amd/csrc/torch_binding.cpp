@@ -586,6 +586,7 @@ std::vector<Tensor> verify_drafts(const Tensor& target_, const std::optional<Ten
   no_gradient(target_, "verify_drafts");
   TORCH_CHECK(target_.dim() == 2 && target_.size(0) < (1LL << 31) && target_.size(1) < (1LL << 31), "fgrpo: target must be [tokens, vocabulary], got ", target_.sizes());
   const int64_t T = target_.size(0), V = target_.size(1);
+  TORCH_CHECK(V > 0, "fgrpo: verify_drafts needs a vocabulary");
   const int code = dtype_code(target_);
   require_one_gpu(target_, ids_, u_, cu_);
   const Tensor cu = index_vector(cu_, target_, "cu_seqlens");
@@ -605,12 +606,13 @@ std::vector<Tensor> verify_drafts(const Tensor& target_, const std::optional<Ten
   const Tensor ids = ids_.reshape({-1}).to(at::kLong).contiguous(), u = per_token(u_, T, "u");
   OnDevice d(target);
   const auto o = target.options().requires_grad(false);
-  Tensor accepted = at::empty({B}, o.dtype(at::kInt)), tokens = at::empty({T}, o.dtype(at::kLong));
-  if (B > 0 && T > 0 && V > 0) {
-    const bool drafts = draft.defined() && draft.size(0) > 0;
+  Tensor accepted = T > 0 ? at::empty({B}, o.dtype(at::kInt)) : at::zeros({B}, o.dtype(at::kInt)), tokens = at::empty({T}, o.dtype(at::kLong));
+  if (B > 0 && T > 0) {
+    const bool drafts = draft.defined(), some = drafts && draft.size(0) > 0;      // a draft of no rows is not none: an address that is not read stands for it
     const Tensor ws = workspace(api.fgrpo_verify_drafts_workspace((int)B, (int)V), target);
-    check(api.fgrpo_verify_drafts(ptr(target), target.stride(0), drafts ? ptr(draft) : nullptr, drafts ? draft.stride(0) : 0, drafts ? (int)draft.size(0) : 0, code, ids.data_ptr<int64_t>(), fptr(u),
-                                  cu.data_ptr<int32_t>(), (int)B, (int)T, (int)V, accepted.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(), ws.data_ptr(), (size_t)ws.numel(), d.stream()), "verify_drafts");
+    check(api.fgrpo_verify_drafts(ptr(target), target.stride(0), drafts ? ptr(some ? draft : target) : nullptr, some ? draft.stride(0) : V, some ? (int)draft.size(0) : 0, code,
+                                  ids.data_ptr<int64_t>(), fptr(u), cu.data_ptr<int32_t>(), (int)B, (int)T, (int)V, accepted.data_ptr<int32_t>(), tokens.data_ptr<int64_t>(),
+                                  ws.data_ptr(), (size_t)ws.numel(), d.stream()), "verify_drafts");
   }
   return {accepted, tokens};
 }

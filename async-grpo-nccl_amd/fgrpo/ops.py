@@ -1217,6 +1217,6 @@ def verify_drafts(target: torch.Tensor, draft: Optional[torch.Tensor], ids: torc
     [drafts, V] those that the drafts were drawn from, a row for each draft in order (None: drafts that were chosen
     outright); bf16 or fp32.  ``u`` [T] in [0, 1): row ``i``'s decides on draft ``i``, and the
     first row whose draft does not stand draws with it.  Returns (how many stand [sequences] int32, tokens [T] int64: those, the
-    one drawn, then -1).  Sums over the vocabulary are held in 64 bits (see ``fgrpo_verify_drafts``)."""
+    one drawn, then -1; rows behind the last sequence hold anything).  Sums over the vocabulary are held in 64 bits (see ``fgrpo_verify_drafts``)."""
     accepted, tokens = _lib.native().verify_drafts(target, draft, ids, u, cu_seqlens)
     return accepted, tokens

@@ -225,6 +225,18 @@ def test_verify_rows_of_any_place_and_values(dev, fp32):
             assert torch.equal(got_a.cpu(), want_a) and torch.equal(got_t.cpu(), want_t)
 
 
+def test_verify_without_rows(dev):
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)      # noqa: E731
+    accepted, tokens = ops.verify_drafts(torch.ones(0, 5, device=dev), None, torch.zeros(0, dtype=torch.long, device=dev), torch.zeros(0, device=dev), i32(0, 0, 0))
+    assert accepted.tolist() == [0, 0] and tokens.numel() == 0
+    # drafts without a row of their distribution count as drawn with probability 0: they stand where the target has anything
+    target = torch.tensor([[0.5, 0.5, 0.0], [0.0, 0.0, 1.0]], device=dev)
+    for last, want in ((0, [1]), (2, [0])):
+        ids, u = torch.tensor([1, last], device=dev), torch.tensor([0.3, 0.3], device=dev)
+        accepted, tokens = ops.verify_drafts(target, torch.zeros(0, 3, device=dev), ids, u, i32(0, 2))
+        assert accepted.tolist() == want and tokens.tolist() == ([0, 2] if want == [1] else [0, -1])
+
+
 def test_callable_with_a_block_table(dev):
     import varlen_attention as VA
     for qs, ks in (([1, 1, 1], [5, 70, 33]), ([60, 200], [60, 333])):

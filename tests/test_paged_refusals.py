@@ -147,3 +147,9 @@ def test_outputs_and_caches_that_want_gradients():
         ops.paged_attention(q, ops.PagedCache(kv, kv.clone().requires_grad_(True)), table, lens, cu)
     with pytest.raises(RuntimeError, match="gradient"):
         ops.paged_cache_write(ops.PagedCache(kv.clone().requires_grad_(True), kv), q[:, :2], q[:, :2], table, lens, cu)
+
+
+def test_verify_needs_a_vocabulary():
+    from fgrpo import ops
+    with pytest.raises(RuntimeError, match="vocabulary"):
+        ops.verify_drafts(torch.zeros(2, 0), None, torch.zeros(2, dtype=torch.long), torch.zeros(2), torch.tensor([0, 2], dtype=torch.int32))
