@@ -78,6 +78,50 @@ def test_one_long_sequence_in_many_parts_and_wrong_hints(dev, n, hint, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("Hq,Hkv,D,block,qs,ks", [
+    (128, 128, 64, 16, [1, 2], [40, 300]),                 # every head its own keys
+    (71, 1, 64, 32, [1, 1, 1], [5, 64, 700]),              # more heads of a group than a block has rows
+    (8, 2, 64, 65536, [3, 1], [70, 1500]),                 # a block longer than any sequence
+    (8, 2, 128, 1024, [2, 90], [1025, 2047])])
+def test_head_counts_and_block_sizes(dev, Hq, Hkv, D, block, qs, ks, fp8):
+    s = _batch(qs, ks, Hq, Hkv, D, block, fp8, seed=31, spare=0)
+    q, table, ln, cu = _dev(s, dev)
+    for hint in (max(qs), 0, 500):
+        out, lse = ops.paged_attention(q, _cache(s, dev), table, ln, cu, return_lse=True, max_len=hint)
+        _check(s, out, lse)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("n", [1, 5, 90])
+def test_a_very_long_sequence(dev, n, fp8):
+    """1.3 million keys, against 64 bits on the device."""
+    L, block, Hq, D = 1300007, 64, 2, 64
+    g = torch.Generator(dev).manual_seed(n)
+    pages = (L + block - 1) // block
+    x = [torch.randn(pages, block, 1, D, generator=g, device=dev).bfloat16() for _ in range(2)]
+    if fp8:
+        a = [t.float().abs().amax(-1) / 448 for t in x]
+        codes = [(t.float() / s[..., None]).to(FP8) for t, s in zip(x, a)]
+        cache, held = ops.PagedCache(*codes, *a), [c.float().double() * s.double()[..., None] for c, s in zip(codes, a)]
+    else:
+        cache, held = ops.PagedCache(*x), [t.double() for t in x]
+    order = torch.randperm(pages, generator=g, device=dev)
+    k, v = (t[order].reshape(-1, D)[:L] for t in held)
+    q = torch.randn(n, Hq, D, generator=g, device=dev).bfloat16()
+    i32 = lambda *y: torch.tensor(y, dtype=torch.int32, device=dev)      # noqa: E731
+    out, lse = ops.paged_attention(q, cache, order[None], i32(L), i32(0, n), return_lse=True, max_len=n)
+    hidden = torch.arange(L - n, L, device=dev)[None, :] > torch.arange(L - n, L, device=dev)[:, None]
+    for h in range(Hq):
+        score = (q[:, h].double() @ k.T) * D ** -0.5
+        score[:, L - n:].masked_fill_(hidden, -math.inf)
+        want = torch.logsumexp(score, 1)
+        score.sub_(want[:, None]).exp_()
+        o, size = score @ v, score @ v.abs()
+        assert ((out[:, h].double() - o).abs() <= 2.0 ** -8 * o.abs() + (2.0 ** -8 + 4e-4) * size).all()
+        assert ((lse[h].double() - want).abs() <= 2e-4 + 2.0 ** -23 * want.abs()).all()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_shared_blocks(dev, fp8):
     """Answers of one prompt read its blocks, each with blocks of its own behind it."""
     Hq, Hkv, D, block, prompt = 6, 2, 128, 16, 64
