@@ -110,7 +110,8 @@ class PagedBatch:
     int32), its length with the new tokens (``seqused_k`` [sequences] int32) and where its new tokens lie in the packed row (``cu_seqlens``
     [sequences + 1] int32).  ``max_len``: the most new tokens of a sequence, 0 where it is not known.  Passed to the model's
     forward as ``paged_batch``, with ``input_ids`` / ``position_ids`` [1, T] and ``use_cache=False``: every attention layer writes its new
-    keys and values and attends over the cache."""
+    keys and values and attends over the cache.  Rows behind the last sequence (a row padded to a fixed length) are written nowhere and come out as
+    anything."""
 
     __slots__ = ("caches", "block_table", "seqused_k", "cu_seqlens", "max_len")
 
