@@ -1,5 +1,5 @@
 // Paged key/value cache, the attention over it and the verification of drafted tokens: C entry points, argument checks and launches
-// (kernels in paged_cache.h, paged_attn.h, draft_kernels.h).
+// (kernels in paged_cache.h, paged_rows.h, paged_tiles.h, paged_deal.h, draft_kernels.h).
 #include <string.h>
 
 #include <algorithm>

@@ -269,6 +269,26 @@ def test_verify_rows_of_any_place_and_values(dev, fp32):
             assert torch.equal(got_a.cpu(), want_a) and torch.equal(got_t.cpu(), want_t)
 
 
+def test_verify_with_offsets_out_of_range(dev):
+    """cu_seqlens that fit nothing are held inside the rows; rows that are right are right."""
+    g = torch.Generator().manual_seed(5)
+    T, V = 9, 300
+    target = torch.randn(T, V, generator=g).softmax(-1)
+    ids, u = torch.randint(0, V, (T,), generator=g), torch.rand(T, generator=g)
+    draft = torch.randn(5, V, generator=g).softmax(-1)
+    for wild in ([0, 3, 2 ** 31 - 1], [0, 3, -4, 9], [9, 5, 0], [-2 ** 31, 3, 2 ** 31 - 1, 0]):
+        cu = torch.tensor(wild, dtype=torch.int32)
+        for d in (None, draft):
+            accepted, tokens = ops.verify_drafts(target.to(dev), None if d is None else d.to(dev), ids.to(dev), u.to(dev), cu.to(dev))
+            accepted = accepted.cpu()
+            assert ((accepted >= 0) & (accepted < T)).all()
+            if wild[:2] == [0, 3]:
+                want_a, want_t = PO.verify(target[:3], d, ids[:3], u[:3], torch.tensor([0, 3]))
+                assert accepted[0] == want_a[0]
+                if wild[2] > 0:
+                    assert torch.equal(tokens.cpu()[:3], want_t)
+
+
 def test_verify_without_rows(dev):
     i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)      # noqa: E731
     accepted, tokens = ops.verify_drafts(torch.ones(0, 5, device=dev), None, torch.zeros(0, dtype=torch.long, device=dev), torch.zeros(0, device=dev), i32(0, 0, 0))
